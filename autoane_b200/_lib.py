@@ -36,6 +36,12 @@ ABI: dict[str, tuple] = {
     "b2p_gemm": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
     "b2p_attention": (i32, [vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, vp]),
     "b2p_attention_backward": (i32, [vp, i32, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp]),
+    "b2p_kv_append": (i32, [vp, vp, i32, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
+    "b2p_kv_read": (i32, [vp, vp, i32, vp, i32, vp, i32, i32, vp]),
+    "b2p_attention_prefix": (i32, [vp, vp, i32, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, vp, i32, i32, vp, szt,
+                                   vp]),
+    "b2p_attention_prefix_workspace": (szt, [i32, i32, i32, i32, i32, i32]),
+    "b2p_sample": (i32, [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "b2p_model_create": (vp, [vp]),
     "b2p_model_free": (None, [vp]),
     "b2p_model_trainable_count": (i64, [vp]),
@@ -120,6 +126,14 @@ class CkptHeader(C.Structure):
         ("cum_wall", C.c_double)] + [(n, C.c_int) for n in ("cum_steps", "cum_batches", "adam_t", "kv_heads",
                                                               "head_dim", "q_dim")]
 
+
+class KVCacheDesc(C.Structure):
+    """b2p_kv_cache (include/b2p.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int) for n in ("n_pages", "page_size", "kv_heads", "kind")]
+
+
+KV_16, KV_INT8, KV_E4M3 = range(3)
 
 CKPT_MAGIC, CKPT_VERSION, LORA_MAGIC = 0x424C5A54, 4, 0x4C4F5241
 

@@ -1,0 +1,263 @@
+"""Decoding on the GPU: a paged key/value cache, attention of a batch whose
+sequences share a long prefix, and sampling.
+
+A thin layer over b2p_kv_append, b2p_kv_read, b2p_attention_prefix and
+b2p_sample (include/b2p.h has their definitions) for torch tensors. All work
+goes to torch's current stream of the tensors' device; nothing synchronises.
+Argument errors raise `B2PError` (from the library) or `ValueError` (shapes and
+types of the tensors). Indices on the device (slots, positions, page ids,
+lengths) are checked there: `check()` raises if any was out of range.
+
+The reference generates with a numpy forward and top-k sampling
+(generate.py:161); a step here is
+
+    q = cache.append(qkv, heads, slots, positions, table)      # rotate, quantise, write
+    y = attend(q, cache, prefix_pages, prefix_len, suffix_pages, suffix_lens)
+    tokens, logprobs = sample(logits, u, temperature, top_k, top_p, min_p)
+
+with the projections between them on b2p_gemm (examples/complete.py).
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from ._lib import KV_16, KV_E4M3, KV_INT8, B2PError, KVCacheDesc
+
+HEAD_DIM = 64
+_DTYPE = {torch.float16: 0, torch.bfloat16: 1}
+_LOGITS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_KIND = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3, torch.float16: KV_16, torch.bfloat16: KV_16}
+
+
+def _fn(name):
+    """The entry point, without argtypes conversion beyond ctypes' own."""
+    return getattr(_lib.load(), name)
+
+
+def _raise(name: str, rc: int):
+    raise B2PError(name, rc, _lib.load().b2p_last_error().decode(errors="replace"))
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _rows(t: torch.Tensor, name: str, dtypes=_DTYPE) -> torch.Tensor:
+    if t.dim() != 2 or t.dtype not in dtypes or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be a CUDA matrix of {[str(d) for d in dtypes]} with contiguous rows")
+    return t
+
+
+def _vec(t, name: str, dtype, n: int, device):
+    """A contiguous vector's address; None gives NULL."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on {device}")
+    return t.data_ptr()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def check(stream: int | None = None) -> None:
+    """Wait for `stream` (default: the current one) and raise if a kernel recorded a bad index or a failed wait."""
+    if stream is None:
+        stream = torch.cuda.current_stream().cuda_stream
+    _lib.call("b2p_device_status", stream)
+
+
+def rope_table(positions: int, rot: int = HEAD_DIM, theta: float = 10000.0, scale: float = 1.0,
+               yarn: tuple[float, float, float] | None = None, device="cuda") -> torch.Tensor:
+    """Cosine and sine of every position's angles, computed in 64 bits: fp32 [positions, rot/2, 2].
+
+    Pair i turns by position·theta^(-2i/rot) (training/cpu_ops.h:303-307). For contexts longer than the training's:
+    `scale` s divides every angle by s (position interpolation); with yarn = (trained_positions, fast, slow) a pair
+    that makes more than `fast` turns over trained_positions keeps its angle, one that makes fewer than `slow` is
+    divided by s, those between are blended linearly in the pair index, and cosines and sines carry the factor
+    0.1·ln(s) + 1 (the attention temperature of that scheme)."""
+    if rot % 16 or not 0 < rot <= HEAD_DIM:
+        raise ValueError(f"rot must be 16, 32, 48 or {HEAD_DIM} (got {rot})")
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    freq = theta ** (-2.0 * i / rot)
+    size = 1.0
+    if yarn is not None:
+        trained, fast, slow = yarn
+        pair = lambda turns: rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot // 2 - 1)
+        blend = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - blend) + freq / scale * blend
+        size = 0.1 * math.log(scale) + 1.0 if scale > 1 else 1.0
+    else:
+        freq = freq / scale
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+    return (torch.stack((angle.cos(), angle.sin()), -1) * size).float().to(device)
+
+
+class KVCache:
+    """A paged cache over the caller's tensors: k and v [n_pages, kv_heads, page_size, 64] of int8, float8_e4m3fn or
+    the compute dtype; 8-bit caches have k_scale and v_scale, fp32 [n_pages, kv_heads, page_size]."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None):
+        if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.dtype not in _KIND or not k.is_cuda:
+            raise ValueError("k must be a CUDA tensor [n_pages, kv_heads, page_size, 64] of int8, float8_e4m3fn, "
+                             "float16 or bfloat16")
+        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError("v must be like k")
+        kind = _KIND[k.dtype]
+        scales = [] if kind == KV_16 else [k_scale, v_scale]
+        for s in scales:
+            if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.device != k.device:
+                raise ValueError("8-bit caches need fp32 k_scale and v_scale [n_pages, kv_heads, page_size]")
+        if not all(t.is_contiguous() for t in (k, v, *scales)):
+            raise ValueError("cache tensors must be contiguous")
+        self.k, self.v = k, v
+        self.k_scale, self.v_scale = scales or (None, None)
+        self.n_pages, self.kv_heads, self.page_size, _ = k.shape
+        self.kind, self.device = kind, k.device
+        self._desc = KVCacheDesc(k.data_ptr(), v.data_ptr(), *(s.data_ptr() for s in scales or ()),
+                                 *((None, None) if not scales else ()), self.n_pages, self.page_size, self.kv_heads,
+                                 kind)
+        self._ref = C.addressof(self._desc)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, kv_heads: int, dtype: torch.dtype = torch.int8,
+              device="cuda") -> "KVCache":
+        """A new cache of `n_pages` pages (uninitialised)."""
+        shape = (n_pages, kv_heads, page_size, HEAD_DIM)
+        new = lambda: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+        scale = (lambda: torch.empty(shape[:3], device=device)) if _KIND.get(dtype) != KV_16 else (lambda: None)
+        return cls(new(), new(), scale(), scale())
+
+    def _dtype(self, dtype: torch.dtype) -> int:
+        if dtype not in _DTYPE or (self.kind == KV_16 and dtype != self.k.dtype):
+            raise ValueError(f"the cache holds {self.k.dtype}: {dtype} does not go with it")
+        return _DTYPE[dtype]
+
+    def append(self, qkv: torch.Tensor, heads: int, slots: torch.Tensor, positions: torch.Tensor | None = None,
+               table: torch.Tensor | None = None, interleaved: bool = False,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Write the K and V of qkv [n, 64·(heads + 2·kv_heads)] to `slots` (int32 [n]; negative: skip), rotated by
+        `table` (see rope_table; None: no rotation) at `positions` (int32 [n]). Returns rotated Q [n, 64·heads]
+        (`out`, which may be a view of qkv)."""
+        _rows(qkv, "qkv")
+        n = qkv.shape[0]
+        if qkv.shape[1] < HEAD_DIM * (heads + 2 * self.kv_heads) or qkv.device != self.device:
+            raise ValueError(f"qkv must have {HEAD_DIM * (heads + 2 * self.kv_heads)} columns, on {self.device}")
+        if out is None:
+            out = torch.empty((n, heads * HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
+        elif out.shape != (n, heads * HEAD_DIM) or out.dtype != qkv.dtype or out.device != qkv.device:
+            raise ValueError(f"out must be {qkv.dtype} [{n}, {heads * HEAD_DIM}] on {qkv.device}")
+        if table is not None and (table.dim() != 3 or table.shape[2] != 2 or positions is None):
+            raise ValueError("table must be [positions, rot/2, 2], and goes with positions")
+        max_pos, rot = (table.shape[0], 2 * table.shape[1]) if table is not None else (0, 0)
+        rc = _fn("b2p_kv_append")(
+            self._ref, qkv.data_ptr(), _ld(qkv), heads, _rows(out, "out").data_ptr(), _ld(out),
+            _vec(slots, "slots", torch.int32, n, self.device),
+            _vec(positions, "positions", torch.int32, n, self.device),
+            None if table is None else _vec(table, "table", torch.float32, max_pos * rot, self.device),
+            max_pos, rot, int(interleaved), n, self._dtype(qkv.dtype), _stream(qkv))
+        if rc:
+            _raise("b2p_kv_append", rc)
+        return out
+
+    def read(self, slots: torch.Tensor, dtype: torch.dtype, k_out: torch.Tensor | None = None,
+             v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The K and V of `slots` (int32 [n]; negative: zeros) as [n, 64·kv_heads] of `dtype`."""
+        n, cols = slots.numel(), HEAD_DIM * self.kv_heads
+        outs = []
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is None:
+                t = torch.empty((n, cols), dtype=dtype, device=self.device)
+            elif t.shape != (n, cols) or t.dtype != dtype or t.device != self.device:
+                raise ValueError(f"{name} must be {dtype} [{n}, {cols}] on {self.device}")
+            outs.append(_rows(t, name))
+        k, v = outs
+        rc = _fn("b2p_kv_read")(self._ref, _vec(slots, "slots", torch.int32, n, self.device), n, k.data_ptr(), _ld(k),
+                                v.data_ptr(), _ld(v), self._dtype(dtype), _stream(slots))
+        if rc:
+            _raise("b2p_kv_read", rc)
+        return k, v
+
+
+class PrefixAttention:
+    """Attention of `batch` sequences with `q_len` queries each over a shared prefix and their own suffixes, with the
+    workspace that calls up to max_prefix and max_suffix tokens need. Calls on one object share it: keep them on one
+    stream, or ordered."""
+
+    def __init__(self, batch: int, q_len: int, heads: int, kv_heads: int, max_prefix: int, max_suffix: int,
+                 device="cuda"):
+        size = _fn("b2p_attention_prefix_workspace")(batch, q_len, heads, kv_heads, max_prefix, max_suffix)
+        if not size:
+            raise ValueError("batch, q_len, heads, kv_heads, max_prefix or max_suffix out of range")
+        self.batch, self.q_len, self.heads, self.kv_heads = batch, q_len, heads, kv_heads
+        self.max_prefix, self.max_suffix = max_prefix, max_suffix
+        self.workspace = torch.zeros(size, dtype=torch.uint8, device=device)
+
+    def __call__(self, q: torch.Tensor, cache: KVCache, prefix_pages: torch.Tensor | None, prefix_len: int,
+                 suffix_pages: torch.Tensor | None, suffix_lens: torch.Tensor | None, out: torch.Tensor | None = None,
+                 return_lse: bool = False):
+        """q [batch·q_len, 64·heads]; prefix_pages int32 [ceil(prefix_len/page_size)]; suffix_pages int32
+        [batch, pages]; suffix_lens int32 [batch] (None: no suffixes). Returns out, or (out, lse [batch·q_len, heads])."""
+        n, dev = self.batch * self.q_len, cache.device
+        _rows(q, "q")
+        if q.shape != (n, self.heads * HEAD_DIM) or q.device != dev or cache.kv_heads != self.kv_heads:
+            raise ValueError(f"q must be [{n}, {self.heads * HEAD_DIM}] on {dev}, the cache have {self.kv_heads} KV heads")
+        if not 0 <= prefix_len <= self.max_prefix:
+            raise ValueError(f"prefix_len must be from 0 to {self.max_prefix}")
+        pages = -(-prefix_len // cache.page_size)
+        if prefix_len and (prefix_pages is None or prefix_pages.numel() < pages):
+            raise ValueError(f"prefix_pages must name {pages} pages")
+        most = self.max_suffix if suffix_lens is not None else 0
+        pitch = 0
+        if most:
+            if suffix_pages is None or suffix_pages.dim() != 2 or suffix_pages.shape[0] != self.batch:
+                raise ValueError("suffix_pages must be [batch, pages]")
+            pitch = suffix_pages.shape[1]
+            most = min(most, pitch * cache.page_size)
+        if out is None:
+            out = torch.empty((n, self.heads * HEAD_DIM), dtype=q.dtype, device=dev)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            raise ValueError("out must be like q")
+        lse = torch.empty((n, self.heads), dtype=torch.float32, device=dev) if return_lse else None
+        i32 = torch.int32
+        rc = _fn("b2p_attention_prefix")(
+            cache._ref, q.data_ptr(), _ld(q), _rows(out, "out").data_ptr(), _ld(out),
+            None if lse is None else lse.data_ptr(), self.batch, self.q_len, self.heads,
+            _vec(prefix_pages, "prefix_pages", i32, prefix_pages.numel(), dev) if prefix_len else None, prefix_len,
+            _vec(suffix_pages, "suffix_pages", i32, self.batch * pitch, dev) if most else None, pitch,
+            _vec(suffix_lens, "suffix_lens", i32, self.batch, dev) if most else None, most,
+            cache._dtype(q.dtype), self.workspace.data_ptr(), self.workspace.numel(), _stream(q))
+        if rc:
+            _raise("b2p_attention_prefix", rc)
+        return (out, lse) if return_lse else out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+           out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """A token for each row of logits [n, vocab] (float16, bfloat16 or float32) from uniform numbers u (fp32 [n]),
+    with per-row temperature, top_p, min_p (fp32 [n]) and top_k (int32 [n]); None turns a filter off. Returns tokens
+    (int32 [n]; `out`) and the natural logs of their probabilities among the kept tokens (fp32 [n])."""
+    _rows(logits, "logits", _LOGITS)
+    n, dev = logits.shape[0], logits.device
+    if out is None:
+        out = torch.empty((n,), dtype=torch.int32, device=dev)
+    logprobs = torch.empty((n,), dtype=torch.float32, device=dev)
+    f32, i32 = torch.float32, torch.int32
+    if u is None:
+        raise ValueError("u is needed")
+    rc = _fn("b2p_sample")(
+        logits.data_ptr(), _ld(logits), n, logits.shape[1], _LOGITS[logits.dtype], _vec(u, "u", f32, n, dev),
+        _vec(temperature, "temperature", f32, n, dev), _vec(top_k, "top_k", i32, n, dev),
+        _vec(top_p, "top_p", f32, n, dev), _vec(min_p, "min_p", f32, n, dev), _vec(out, "out", i32, n, dev),
+        logprobs.data_ptr(), _stream(logits))
+    if rc:
+        _raise("b2p_sample", rc)
+    return out, logprobs

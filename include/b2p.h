@@ -126,6 +126,109 @@ int b2p_attention_backward(const void* qkv, int ld_qkv, const void* out, const v
                            float rope_theta, int dtype, void* stream);
 
 /* ======================================================================
+ * Decoding: a paged key/value cache, attention of a batch that shares a long
+ * prefix, and sampling. The reference generates text with a numpy forward and
+ * top-k sampling (generate.py:161); these are the device operators of such
+ * a loop. All take device pointers, are asynchronous on `stream` and allocate
+ * nothing. head_dim is 64, as in every model here.
+ *
+ * Indices that live on the device (slots, positions, page ids, lengths) are
+ * checked by the kernels: an entry out of range is skipped and recorded, and
+ * b2p_device_status then returns B2P_ERR_DEVICE.
+ * ====================================================================== */
+#define B2P_KV_16 0   /* keys and values in the compute dtype, no scales */
+#define B2P_KV_INT8 1 /* int8 codes, one fp32 scale per token and KV head */
+#define B2P_KV_E4M3 2 /* fp8 e4m3 codes, one fp32 scale per token and KV head */
+
+/* A paged cache. Slot s of the cache is entry s % page_size of page
+ * s / page_size; which page holds which tokens is the caller's page list.
+ * Within a page the tokens of one KV head are contiguous. page_size is a power
+ * of two from 8 to 1024; n_pages * page_size < 2^31. Code pointers are 16-byte
+ * aligned, scale pointers 8-byte aligned. */
+typedef struct {
+  void* k;        /* [n_pages][kv_heads][page_size][64] codes */
+  void* v;        /* the same */
+  float* k_scale; /* [n_pages][kv_heads][page_size]; NULL for B2P_KV_16 */
+  float* v_scale;
+  int n_pages, page_size, kv_heads;
+  int kind;       /* B2P_KV_* */
+} b2p_kv_cache;
+
+/* Write n_tokens new tokens into the cache. qkv [n_tokens][ld_qkv] holds a
+ * token's Q (64*heads columns), K (64*kv_heads) and V (64*kv_heads), as the
+ * fused QKV projection leaves them, before rotation.
+ *   - Q and K are rotated by the angles of the token's position: rope is fp32
+ *     [max_pos][rot/2][2] (cosine, sine), `rot` (0, 16, 32, 48 or 64) the number
+ *     of leading channels of a head that rotate, in pairs (i, i + rot/2), or
+ *     (2i, 2i+1) with interleaved = 1 (apply_rope, generate.py:110). Scaling for
+ *     long contexts is in the table. rot = 0: no rotation, rope may be NULL.
+ *   - Rotated Q goes to q_out [n_tokens][ld_q] in the compute dtype (q_out may
+ *     be qkv itself, with ld_q = ld_qkv).
+ *   - K and V go to slot slots[t]; a negative slot skips the token's K and V.
+ *     Two tokens of one call may not name the same slot.
+ * 8-bit kinds: with A the largest |x| of a (token, head) vector, taken in fp32
+ * after rotation, codes are x * (c / max(A, 1e-30)) rounded to nearest even
+ * (c = 127 for int8, 448 for e4m3) and the scale is max(A, 1e-30) / c. A vector
+ * with a non-finite value reads back as NaN. */
+int b2p_kv_append(const b2p_kv_cache* cache, const void* qkv, int ld_qkv, int heads, void* q_out, int ld_q,
+                  const int32_t* slots, const int32_t* positions, const float* rope, int max_pos, int rot,
+                  int interleaved, int n_tokens, int dtype, void* stream);
+
+/* Read n_tokens slots back: code * scale, rounded to the compute dtype, into
+ * k_out [n_tokens][ld_k] and v_out [n_tokens][ld_v] (64*kv_heads columns; they
+ * may be the K and V columns of a token-major Q|K|V buffer, the form
+ * b2p_attention reads). A negative slot gives zeros. */
+int b2p_kv_read(const b2p_kv_cache* cache, const int32_t* slots, int n_tokens, void* k_out, int ld_k, void* v_out,
+                int ld_v, int dtype, void* stream);
+
+/* Attention of `batch` sequences that share the first prefix_len cached tokens.
+ * Each has q_len queries, its last q_len tokens: q [batch*q_len][ld_q], rotated,
+ * 64*heads columns. Query i of sequence b sees the whole prefix, held in the
+ * slots of prefix_pages [ceil(prefix_len/page_size)], and the first
+ * max(0, suffix_lens[b] - (q_len-1-i)) tokens of its own suffix, held in the
+ * slots of suffix_pages [batch][suffix_pitch] (suffix_lens counts the queries'
+ * own tokens, already appended). The prefix is read once for the whole batch.
+ *   out [batch*q_len][ld_out]: softmax(q·Kᵀ/8)·V in the compute dtype
+ *   lse (may be NULL) fp32 [batch*q_len][heads]: log2 of the sum of exp, as in
+ *       b2p_attention: max·log2(e)/8 + log2(sum)
+ * A query that sees nothing gets zeros and -inf. suffix_lens lives on the
+ * device; max_suffix bounds its entries and suffix_pitch >=
+ * ceil(max_suffix/page_size). Query head h reads KV head h / (heads/kv_heads).
+ * `workspace` holds at least b2p_attention_prefix_workspace() bytes (16-byte
+ * aligned) for sizes that are at least this call's in each argument; calls that
+ * share one must be ordered by their stream. Results repeat bit for bit. */
+int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, void* out, int ld_out, float* lse,
+                         int batch, int q_len, int heads, const int32_t* prefix_pages, int prefix_len,
+                         const int32_t* suffix_pages, int suffix_pitch, const int32_t* suffix_lens, int max_suffix,
+                         int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* Workspace bytes of b2p_attention_prefix (0 for sizes it rejects). */
+size_t b2p_attention_prefix_workspace(int batch, int q_len, int heads, int kv_heads, int prefix_len, int max_suffix);
+
+#define B2P_F32 2 /* b2p_sample only: 32-bit logits */
+
+/* Sample one token per row of logits [rows][ld] (`vocab` columns; dtype B2P_F16,
+ * B2P_BF16 or B2P_F32) from given uniform numbers u [rows] in [0, 1). The
+ * per-row parameters are device arrays; NULL turns one off:
+ *   temperature [rows] (<= 0: the likeliest token), top_k [rows] (<= 0: off),
+ *   top_p [rows] (>= 1: off), min_p [rows] (<= 0: off).
+ * With m the row's largest logit, token j has the depth
+ *   d_j = min((m - x_j)·(log2(e)/T), 64) below it, in steps of 2^-20, and the
+ *   integer weight w_j = 2^31·2^-d_j rounded to nearest, so that sums do not
+ * depend on their order and a draw repeats bit for bit. Tokens are ranked by
+ * depth, ties by index. Kept are: the first top_k; of those, each whose
+ * preceding weights sum to less than top_p times the sum of the kept; of those,
+ * each with w >= min_p·2^31; the first one always. The token drawn is the first
+ * (in index order) at which the running sum of kept weights exceeds
+ * u·(their sum).
+ *   tokens [rows]; logprobs (may be NULL) fp32 [rows]: the natural log of the
+ *   drawn token's probability among the kept.
+ * NaN and -inf logits are never drawn (NaN counts as -inf); +inf logits share
+ * the draw. A row with no token to draw gets -1 and NaN. vocab < 2^21. */
+int b2p_sample(const void* logits, int ld, int rows, int vocab, int dtype, const float* u, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+               void* stream);
+
+/* ======================================================================
  * Device-resident model: the MeZO-LoRA-split hot path on the GPU.
  *
  * Replaces the per-layer compile/stage/eval/read round trips of
