@@ -34,8 +34,8 @@ constexpr int kStep = 32;            // keys of one warp step
 constexpr int kMaxChunk = 4096;      // keys of one part
 constexpr int kMaxChunkPages = kMaxChunk / 8 + 1;
 constexpr int kMinPart = 128;        // no part shorter: its join would cost what it saves
-constexpr int kWant = 148 * 4;       // blocks wanted of each list
-constexpr int kTileRows = 32;        // most rows of a block
+constexpr int kWant = kSms * 4;      // blocks wanted of each list
+constexpr int kTcRows = 64;          // rows from which the prefix goes to the tcgen05 kernel
 
 __device__ __forceinline__ float exp2_sfu(float x) {
   float y;
@@ -113,11 +113,16 @@ __device__ __forceinline__ void load_step(StepRegs<KIND>& r, const KvView& c, co
 
 template <typename T, int KIND, int MT>
 __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles,
-                                                                int prefix_units, uint32_t* status) {
+                                                                int prefix_units, int overlap, uint32_t* status) {
   __shared__ int s_pages[kMaxChunkPages];
   __shared__ __align__(16) float s_o[kRowWarps][MT * 16][kKvHeadDim];
   __shared__ float2 s_ml[kRowWarps][MT * 16];
-  pdl_enter();
+  // After the tcgen05 kernel of the same call (overlap) the inputs are complete already and no part is shared with
+  // it: this kernel then waits for it only at the end, so that whoever waits for this one has both.
+  if (overlap)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  else
+    pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y;
   int u = blockIdx.x;
@@ -137,14 +142,17 @@ __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, in
     const int per = a.n_suffix * suffix_tiles;
     const int b = u / per, s = (u % per) / suffix_tiles, tile = u % suffix_tiles;
     const int span = a.q_len * a.group;
-    part = a.n_prefix + s;
+    part = a.suffix_part + s;
     row0 = b * span + tile * MT * 16;
     row_end = min((b + 1) * span, row0 + MT * 16);
     first = s * a.suffix_chunk;
     base_len = suffix_len(a, b, status);
     end = min(base_len, first + a.suffix_chunk);
     list = a.suffix_pages + (long long)b * a.suffix_pitch;
-    if (first >= end) return;
+    if (first >= end) {
+      if (overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
+      return;
+    }
   }
   const int sh = a.c.page_shift;
   for (int i = threadIdx.x; i <= ((end - 1) >> sh) - (first >> sh); i += kRowThreads) {
@@ -342,6 +350,7 @@ __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, in
     *reinterpret_cast<float4*>(a.part_o + at * kKvHeadDim + d) = acc;
     if (d == 0) a.part_ml[at] = make_float2(top, sum);
   }
+  if (overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // One half-warp per row: join the row's parts, normalise, round.
@@ -354,18 +363,20 @@ __global__ void __launch_bounds__(128) attn_join_kernel(PrefixArgs a, uint32_t* 
   const int token = r / a.group;
   const int len = a.max_suffix > 0 ? suffix_len(a, token / a.q_len, status) : 0;
   const int used = a.max_suffix > 0 ? (len + a.suffix_chunk - 1) / a.suffix_chunk : 0;
-  const int parts = a.n_prefix + used;
+  const int shared = r < a.pair_rows ? a.n_prefix : a.n_last;
+  const int parts = shared + used;
+  auto part = [&](int p) { return p < shared ? p : p - shared + a.suffix_part; };
   const long long stride = (long long)heads_kv * a.rows, at0 = (long long)kvh * a.rows + r;
   float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * stride + at0].x);
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[part(p) * stride + at0].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[p * stride + at0];
+    const float2 ml = a.part_ml[part(p) * stride + at0];
     const float f = exp2_sfu(ml.x - ref);
     sum += f * ml.y;
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p * stride + at0) * kKvHeadDim + d);
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (part(p) * stride + at0) * kKvHeadDim + d);
     acc.x += f * x.x;
     acc.y += f * x.y;
     acc.z += f * x.z;
@@ -383,7 +394,10 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 // How the work is divided: about four blocks for each SM, no part shorter than kMinPart keys nor
 // longer than the page list that a block keeps.
 struct Plan {
-  int mt, prefix_tiles, suffix_tiles, n_prefix, prefix_chunk, n_suffix, suffix_chunk;
+  bool tc;  // the prefix goes to the tcgen05 kernel
+  int mt, prefix_tiles, suffix_tiles, n_suffix, suffix_chunk;
+  PrefixSplit split;
+  int suffix_part, parts;
 };
 int chunk_for(int len, int tiles, int want) {
   int n = ceil_div(want, tiles);
@@ -396,27 +410,33 @@ int chunk_for(int len, int tiles, int want) {
 Plan make_plan(int batch, int q_len, int group, int kv_heads, int prefix_len, int max_suffix) {
   Plan p = {};
   const int rows = batch * q_len * group;
-  p.mt = rows > 16 && prefix_len > 0 ? 2 : 1;
+  p.tc = prefix_len > 0 && rows >= kTcRows;
+  p.mt = (p.tc || prefix_len == 0 ? q_len * group : rows) > 16 ? 2 : 1;
   p.prefix_tiles = ceil_div(rows, 16 * p.mt);
   p.suffix_tiles = ceil_div(q_len * group, 16 * p.mt);
-  if (prefix_len > 0) {
-    p.prefix_chunk = chunk_for(prefix_len, p.prefix_tiles * kv_heads, kWant);
-    p.n_prefix = ceil_div(prefix_len, p.prefix_chunk);
+  p.split.pair_rows = rows;
+  if (p.tc) {
+    prefix_tc_plan(rows, kv_heads, prefix_len, &p.split);
+  } else if (prefix_len > 0) {
+    p.split.prefix_chunk = chunk_for(prefix_len, p.prefix_tiles * kv_heads, kWant);
+    p.split.n_prefix = ceil_div(prefix_len, p.split.prefix_chunk);
   }
   if (max_suffix > 0) {
     p.suffix_chunk = chunk_for(max_suffix, batch * p.suffix_tiles * kv_heads, kWant);
     p.n_suffix = ceil_div(max_suffix, p.suffix_chunk);
   }
+  p.suffix_part = p.split.n_prefix > p.split.n_last ? p.split.n_prefix : p.split.n_last;
+  p.parts = p.suffix_part + p.n_suffix;
   return p;
 }
 
 template <typename T, int KIND, int MT>
 int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
-  const long long prefix_units = (long long)p.n_prefix * p.prefix_tiles;
+  const long long prefix_units = p.tc ? 0 : (long long)p.split.n_prefix * p.prefix_tiles;
   const long long units = prefix_units + (long long)a.batch * p.n_suffix * p.suffix_tiles;
   B2P_REQUIRE(units < (1ll << 31), "too much work for one call");
   B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT>, dim3((unsigned)units, a.c.kv_heads), dim3(kRowThreads), 0,
-                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, c->status));
+                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, p.tc ? 1 : 0, c->status));
   B2P_POST_LAUNCH();
   return B2P_OK;
 }
@@ -424,7 +444,9 @@ int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStre
 template <typename T, int KIND>
 int run_t(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   int rc = B2P_OK;
-  if (p.n_prefix + p.n_suffix > 0)
+  if (p.tc) rc = launch_prefix_tc(a, std::is_same<T, __nv_bfloat16>::value, st);
+  if (rc) return rc;
+  if (p.n_suffix > 0 || (p.split.n_prefix > 0 && !p.tc))
     rc = p.mt == 2 ? launch_rows<T, KIND, 2>(a, p, c, st) : launch_rows<T, KIND, 1>(a, p, c, st);
   if (rc) return rc;
   B2P_CHECK_CUDA(launch_pdl(attn_join_kernel<T>, dim3(ceil_div(a.rows, 8), a.c.kv_heads), dim3(128), 0, st, a,
@@ -461,13 +483,13 @@ extern "C" {
 size_t b2p_attention_prefix_workspace(int batch, int q_len, int heads, int kv_heads, int prefix_len, int max_suffix) {
   if (!sizes_ok(batch, q_len, heads, kv_heads, prefix_len, max_suffix)) return 0;
   // A bound that grows with every argument, so that the workspace of the largest call serves all: parts are
-  // kMinPart keys or longer, and there are about kWant blocks of at most kTileRows rows, or one per kMaxChunk keys.
+  // kTcStageKeys keys or longer, and there are about kWant blocks of 32 rows, or kSms of 256, or one per kMaxChunk keys.
   const long long rows = (long long)batch * q_len * heads;
   long long slots = 0;
   for (int len : {prefix_len, max_suffix}) {
     if (len == 0) continue;
-    const long long by_length = rows * ceil_div(len, kMinPart);
-    const long long by_blocks = (long long)kTileRows * kWant + rows * (2 + len / kMaxChunk);
+    const long long by_length = rows * ceil_div(len, kTcStageKeys);
+    const long long by_blocks = (long long)kSms * 256 + rows * (2 + len / kMaxChunk);
     slots += by_length < by_blocks ? by_length : by_blocks;
   }
   return (size_t)slots * (kKvHeadDim * sizeof(float) + sizeof(float2)) + 256;
@@ -501,7 +523,7 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   B2P_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
   const int group = heads / a.c.kv_heads;
   const Plan p = make_plan(batch, q_len, group, a.c.kv_heads, prefix_len, max_suffix);
-  const size_t uses = (size_t)(p.n_prefix + p.n_suffix) * batch * q_len * heads * (kKvHeadDim * 4 + sizeof(float2));
+  const size_t uses = (size_t)p.parts * batch * q_len * heads * (kKvHeadDim * 4 + sizeof(float2));
   B2P_REQUIRE(uses <= workspace_bytes, "workspace bound of %zu bytes does not hold %zu", need, uses);
   DeviceCtx* c = nullptr;
   if ((rc = ctx_get(&c))) return rc;
@@ -514,7 +536,7 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   a.rows = batch * q_len * group;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o +
-                                        (size_t)(p.n_prefix + p.n_suffix) * a.rows * a.c.kv_heads * kKvHeadDim);
+                                        (size_t)p.parts * a.rows * a.c.kv_heads * kKvHeadDim);
   a.ld_q = ld_q;
   a.ld_out = ld_out;
   a.batch = batch;
@@ -523,8 +545,8 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   a.prefix_len = prefix_len;
   a.suffix_pitch = suffix_pitch;
   a.max_suffix = max_suffix;
-  a.n_prefix = p.n_prefix;
-  a.prefix_chunk = p.prefix_chunk;
+  static_cast<PrefixSplit&>(a) = p.split;
+  a.suffix_part = p.suffix_part;
   a.n_suffix = p.n_suffix;
   a.suffix_chunk = p.suffix_chunk;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

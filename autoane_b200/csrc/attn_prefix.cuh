@@ -7,9 +7,15 @@ namespace b2p {
 
 // Rows of one KV head: r = (b * q_len + i) * group + g, for query i of sequence b and query head
 // kvh * group + g. A part is what one kernel block computes for some rows over some keys: the rows'
-// maximum score (log2 domain), sum of exponentials and unnormalised output. Parts 0 .. n_prefix - 1 split
-// the prefix, the others each sequence's suffix, every split a fixed number of keys.
-struct PrefixArgs {
+// maximum score (log2 domain), sum of exponentials and unnormalised output. The first parts split the
+// prefix, those from max(n_prefix, n_last) on each sequence's suffix, every split a fixed number of keys.
+struct PrefixSplit {
+  int pair_rows;               // rows below it: n_prefix parts of prefix_chunk keys
+  int n_prefix, prefix_chunk;
+  int n_last, last_chunk;      // rows from it on: n_last parts of last_chunk keys
+};
+
+struct PrefixArgs : PrefixSplit {
   KvView c;
   const void* q;
   void* out;
@@ -22,10 +28,16 @@ struct PrefixArgs {
   long long ld_q, ld_out;
   int batch, q_len, group, rows;  // rows = batch * q_len * group, of one KV head
   int prefix_len, suffix_pitch, max_suffix;
-  int n_prefix, prefix_chunk;  // prefix parts and keys of each
+  int suffix_part;             // first part of a suffix
   int n_suffix, suffix_chunk;  // suffix parts and keys of each
 };
 
+// The prefix part on the tcgen05 tensor cores (attn_prefix_tc.cu), and its division of the prefix.
+int launch_prefix_tc(const PrefixArgs& a, bool bf16, cudaStream_t st);
+void prefix_tc_plan(int rows, int kv_heads, int prefix_len, PrefixSplit* s);
+
+constexpr int kTcStageKeys = 128;  // its parts are multiples of this many keys
+constexpr int kSms = 148;  // of a B200: what the work divisions aim at
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 1/sqrt(64) * log2(e)
 
 // The length of sequence b's suffix (a bad entry counts as empty and is recorded).
