@@ -9,17 +9,18 @@
 // each sequence's suffix is another.
 //
 // attn_rows_kernel: each warp holds 16 or 32 query rows of one KV head and runs
-// over 32 keys at a time with mma.sync. Keys and values go from global memory
-// straight into the registers of the fragment: a head's 64 channels are taken in
-// the order that gives each thread 16 consecutive ones of a key (S = Q·Kᵀ sums
-// over channels, so Q is read in the same order) and 8 consecutive ones of a
-// value (each is a column of O of its own).
+// over 32 keys at a time with mma.sync. Its keys and values come as they are
+// stored into a ring of its own in shared memory (cp.async, up to 128 keys ahead,
+// no barrier between warps) and from there into fragments: a head's 64 channels
+// are taken in the order that gives each thread 16 consecutive ones of a key
+// (S = Q·Kᵀ sums over channels, so Q is read in the same order) and 8 consecutive
+// ones of a value (each is a column of O of its own).
 //
 // 8-bit caches: codes widen to 16 bit exactly. A key's scale multiplies its
 // column of S in fp32. A value's scale y_j joins the exponent,
-//   w_j = exp2(s_j log2e + log2 y_j - M), M the running maximum of the sum,
+//   w_j = exp2(s_j log2e + log2 y_j - M), M near the largest of the sums so far,
 // so that o = sum w_j code_j, l = sum w_j / y_j and out = o / l: the one rounding
-// to 16 bit is that of w_j <= 1, as without scales, however small the values are.
+// to 16 bit is that of w_j, as without scales, however small the values are.
 #include <cstdint>
 #include <type_traits>
 #include "attn_prefix.cuh"
@@ -31,33 +32,62 @@ namespace {
 constexpr int kRowWarps = 4;
 constexpr int kRowThreads = kRowWarps * 32;
 constexpr int kStep = 32;            // keys of one warp step
+constexpr int kPitch = kKvHeadDim + 4;  // floats of a row of O in shared memory
 constexpr int kMaxChunk = 4096;      // keys of one part
 constexpr int kMaxChunkPages = kMaxChunk / 8 + 1;
+constexpr int kTeamOneKeys = 2048;   // suffixes up to this go to single warps, in units of 128 or 256 keys
+constexpr float kSlack = 8.f;        // weights go up to 2^8 before a row's reference moves
 constexpr int kMinPart = 128;        // no part shorter: its join would cost what it saves
 constexpr int kWant = kSms * 4;      // blocks wanted of each list
 constexpr int kTcRows = 64;          // rows from which the prefix goes to the tcgen05 kernel
 
-__device__ __forceinline__ float exp2_sfu(float x) {
+__device__ __forceinline__ float rcp_sfu(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
 __device__ __forceinline__ float log2_sfu(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Keys of one step as loaded: n8 tiles j = 0..3 of 8 keys each.
+// A step's keys in shared memory: K rows, V rows (16-byte chunks of a row exchanged so that the fragments' reads meet
+// no bank conflict), and for 8-bit kinds the scales of 32 keys and 32 values.
 template <int KIND>
-struct StepRegs {
-  static constexpr int kKW = KIND == B2P_KV_16 ? 8 : 4;  // words of a thread's 16 channels of a key
-  static constexpr int kVW = KIND == B2P_KV_16 ? 4 : 2;  // words of its 8 channels of a value
-  uint32_t k[4][kKW];
-  uint32_t v[4][2][kVW];
-  float2 ks[4], vs[4];
+struct StepMem {
+  static constexpr bool kQ8 = KIND != B2P_KV_16;
+  static constexpr int kRow = kQ8 ? 64 : 128;        // bytes of a key
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kV = kStep * kRow;            // offset of V, then of the scales
+  static constexpr int kScale = 2 * kStep * kRow;
+  static constexpr int kBytes = kScale + (kQ8 ? 2 * kStep * 4 : 0);
+  static constexpr int kRing = kQ8 ? 4 : 2;          // steps of a warp's ring
+  static constexpr int kBlock = kRowWarps * kRing * kBytes;
+  static __device__ __forceinline__ int k_at(int key, int chunk) {
+    return key * kRow + (kQ8 ? chunk : chunk ^ (key & 7)) * 16;
+  }
+  static __device__ __forceinline__ int v_at(int key, int chunk) {
+    return kV + key * kRow + (kQ8 ? chunk ^ ((key >> 1) & 3) : chunk ^ (key & 7)) * 16;
+  }
 };
+
+__device__ __forceinline__ void cp_async_or_zero16(uint32_t saddr, const void* g, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(g), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_or_zero4(uint32_t saddr, const void* g, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(saddr), "l"(g), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
 
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
@@ -77,114 +107,129 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
   }
 }
 
-// Load the 32 keys from key0 (a multiple of 8 inside the list) on; keys from `end` on give zeros.
-// pages[] is the part's page list in shared memory, its first page holding key `first`.
-template <int KIND>
-__device__ __forceinline__ void load_step(StepRegs<KIND>& r, const KvView& c, const int* pages, int first, int kvh,
-                                          int key0, int end, int g, int t) {
-  constexpr int kBytes = KIND == B2P_KV_16 ? 128 : 64;  // of a key
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int key = key0 + 8 * j;
-#pragma unroll
-    for (int i = 0; i < StepRegs<KIND>::kKW; ++i) r.k[j][i] = 0;
-#pragma unroll
-    for (int i = 0; i < StepRegs<KIND>::kVW; ++i) r.v[j][0][i] = r.v[j][1][i] = 0;
-    r.ks[j] = make_float2(0.f, 0.f);
-    r.vs[j] = make_float2(1.f, 1.f);
-    if (key >= end) continue;
-    const int page = pages[(key >> c.page_shift) - (first >> c.page_shift)];
-    if (page < 0) continue;
-    const long long at = c.vec(page, kvh, key & ((1 << c.page_shift) - 1));
-    if (key + g < end) load_words(r.k[j], c.k + (at + g) * kBytes + t * (kBytes / 4));
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int kk = 2 * t + e;
-      if (key + kk < end) {
-        load_words(r.v[j][e], c.v + (at + kk) * kBytes + g * (kBytes / 8));
-        if (KIND != B2P_KV_16) {
-          (e ? r.ks[j].y : r.ks[j].x) = __ldg(c.k_scale + at + kk);
-          (e ? r.vs[j].y : r.vs[j].x) = __ldg(c.v_scale + at + kk);
-        }
-      }
-    }
-  }
-}
-
-template <typename T, int KIND, int MT>
-__global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles,
-                                                                int prefix_units, int overlap, uint32_t* status) {
-  __shared__ int s_pages[kMaxChunkPages];
-  __shared__ __align__(16) float s_o[kRowWarps][MT * 16][kKvHeadDim];
-  __shared__ float2 s_ml[kRowWarps][MT * 16];
-  // After the tcgen05 kernel of the same call (overlap) the inputs are complete already and no part is shared with
-  // it: this kernel then waits for it only at the end, so that whoever waits for this one has both.
-  if (overlap)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  else
+// W warps share a unit of work (some rows, some keys): 1 where sequences are many and short, so that no warp waits
+// for another, else the block's 4, whose parts are joined in shared memory first. 
+template <typename T, int KIND, int MT, int W, bool FUSE>
+__global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
+    attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status) {
+  extern __shared__ __align__(16) uint8_t s_ring[];
+  using Mem = StepMem<KIND>;
+  __shared__ int s_pages[W == 1 ? 1 : kMaxChunkPages];
+  __shared__ __align__(16) float s_o[W == 1 ? 1 : W][W == 1 ? 1 : MT * 16][kPitch];
+  __shared__ float2 s_ml[W][MT * 16];
+  __shared__ int s_last[MT * 16];
+  // After the tcgen05 kernel of the same call (!FUSE) the inputs are complete already and no part is shared with it:
+  // this kernel then waits for it only at the end, so that the join, which waits for this one, has both.
+  if (FUSE)
     pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  else
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = W == 1 ? 0 : threadIdx.x >> 5;  // in the team
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y;
-  int u = blockIdx.x;
-  // this block's rows [row0, row_end), keys [first, end), page list and part
-  int row0, row_end, first, end, part;
-  int base_len = 1 << 30;  // keys that the last query of the rows' sequence sees
+  int u = W == 1 ? blockIdx.x * kRowWarps + (threadIdx.x >> 5) : blockIdx.x;
+  if (W == 1 && u >= units) {
+    if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  // this unit's rows [row0, row_end), keys [first, end), page list and part
+  const int span = a.q_len * a.group;
+  int row0, row_end, first, end, part, b = 0;
+  int len = 0;             // of the suffix of the rows' sequence
+  int base_len = 1 << 30;  // keys that its last query sees
   const int32_t* list;
-  if (u < prefix_units) {
-    part = u / prefix_tiles;
-    row0 = (u % prefix_tiles) * MT * 16;
+  const bool shared = u < prefix_units;
+  if (shared) {
+    part = prefix_tiles == 1 ? u : u / prefix_tiles;
+    row0 = (u - part * prefix_tiles) * MT * 16;
     row_end = min(a.rows, row0 + MT * 16);
     first = part * a.prefix_chunk;
     end = min(a.prefix_len, first + a.prefix_chunk);
     list = a.prefix_pages;
   } else {
     u -= prefix_units;
-    const int per = a.n_suffix * suffix_tiles;
-    const int b = u / per, s = (u % per) / suffix_tiles, tile = u % suffix_tiles;
-    const int span = a.q_len * a.group;
+    b = u / (a.n_suffix * suffix_tiles);
+    u -= b * a.n_suffix * suffix_tiles;
+    const int s = suffix_tiles == 1 ? u : u / suffix_tiles, tile = u - s * suffix_tiles;
     part = a.suffix_part + s;
     row0 = b * span + tile * MT * 16;
     row_end = min((b + 1) * span, row0 + MT * 16);
     first = s * a.suffix_chunk;
-    base_len = suffix_len(a, b, status);
-    end = min(base_len, first + a.suffix_chunk);
+    end = min(a.max_suffix, first + a.suffix_chunk);  // (until the length is here)
     list = a.suffix_pages + (long long)b * a.suffix_pitch;
-    if (first >= end) {
-      if (overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
-      return;
-    }
+    len = suffix_len(a, b, status);
   }
+  // the page list, the length and Q come together
   const int sh = a.c.page_shift;
-  for (int i = threadIdx.x; i <= ((end - 1) >> sh) - (first >> sh); i += kRowThreads) {
-    int p = list[(first >> sh) + i];
-    if (p < 0 || p >= a.c.n_pages) {
-      atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
-      p = -1;
-    }
-    s_pages[i] = p;
+  const int pages = ((end - 1) >> sh) - (first >> sh) + 1;
+  int my_page = 0;  // (W 1: 256 keys at most, so 32 pages)
+  if (W == 1) {
+    if (lane < pages) my_page = list[(first >> sh) + lane];
+  } else {
+    for (int i = threadIdx.x; i < pages; i += kRowThreads) s_pages[i] = list[(first >> sh) + i];
   }
-  __syncthreads();
+  // a page that the list has wrong: recorded, page 0 in its place
+  auto checked = [&](int page, bool used) {
+    const bool bad = (unsigned)page >= (unsigned)a.c.n_pages;
+    if (bad && used) atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
+    return bad ? 0 : page;
+  };
 
-  // Q fragments and the number of keys that each of the thread's rows sees
-  uint32_t q[MT][2][8];
+  // Q fragments and the number of keys that each of the thread's rows sees (rows that do not exist see all)
+  uint32_t q[MT][4][4];  // A fragments, [k step]
   int lim[MT][2];
-  int min_lim = 1 << 30;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = row0 + m * 16 + e * 8 + g;
-      lim[m][e] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[m][e][i] = 0;
+      lim[m][e] = 1 << 30;
+      uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       if (r < row_end) {
-        const T* src = static_cast<const T*>(a.q) + (long long)(r / a.group) * a.ld_q +
-                       (kvh * a.group + r % a.group) * kKvHeadDim + t * 16;
-        load_words(q[m][e], reinterpret_cast<const uint8_t*>(src));
-        lim[m][e] = min(end, base_len - (a.q_len - 1 - (r / a.group) % a.q_len));
+        const int token = r / a.group;
+        const T* src = static_cast<const T*>(a.q) + (long long)token * a.ld_q +
+                       (kvh * a.group + r - token * a.group) * kKvHeadDim + t * 16;
+        load_words(w, reinterpret_cast<const uint8_t*>(src));
+        if (!shared) lim[m][e] = (b + 1) * a.q_len - 1 - token;  // later queries: taken off the length below
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        q[m][k][e] = w[2 * k];
+        q[m][k][2 + e] = w[2 * k + 1];
+      }
+    }
+  if (!shared) {
+    base_len = len;
+    end = min(end, len);
+    if (first >= end) {
+      // No key here: another part's unit writes the rows, or, where there is none, the first suffix unit does.
+      if (first == 0 && a.suffix_part == 0)
+        for (int r = row0 + (W == 1 ? lane >> 4 : threadIdx.x >> 4); r < row_end; r += 2 * W)
+          join_row<T>(a, kvh, r, 0, threadIdx.x & 15);
+      if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
+      return;
+    }
+  }
+  int min_lim = 1 << 30;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (shared)
+        lim[m][e] = end;
+      else if (lim[m][e] < (1 << 30))
+        lim[m][e] = min(end, base_len - lim[m][e]);
+      else
+        lim[m][e] = end;
       min_lim = min(min_lim, lim[m][e]);
     }
+  const int used_pages = ((end - 1) >> sh) - (first >> sh) + 1;
+  if (W == 1) {
+    my_page = checked(my_page, lane < used_pages);
+  } else {  // (each thread checks what it loaded)
+    for (int i = threadIdx.x; i < used_pages; i += kRowThreads) s_pages[i] = checked(s_pages[i], true);
+    __syncthreads();
+  }
 
   float o[MT][8][4];
   float mx[MT][2], l[MT][2];
@@ -196,77 +241,94 @@ __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, in
     for (int n = 0; n < 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
   }
 
-  StepRegs<KIND> cur;
-  int key0 = first + warp * kStep;
-  if (key0 < end) load_step<KIND>(cur, a.c, s_pages, first, kvh, key0, end, g, t);
-  for (; key0 < end; key0 += kRowWarps * kStep) {
+  const uint32_t ring = smem_u32(s_ring) + (threadIdx.x >> 5) * (Mem::kRing * Mem::kBytes);
+  const uint32_t page_vecs = (uint32_t)a.c.kv_heads << sh;  // vectors of a page
+  const uint8_t* k0 = a.c.k + ((long long)kvh << sh) * Mem::kRow + lane * 16;
+  const uint8_t* v0 = a.c.v + ((long long)kvh << sh) * Mem::kRow + lane * 16;
+  auto page_of = [&](int key) {
+    const int at = (min(key, end - 1) >> sh) - (first >> sh);
+    return (uint32_t)(W == 1 ? __shfl_sync(~0u, my_page, at) : s_pages[at]);
+  };
+  // Step i of this warp: keys from first + (warp + i·W)·32 on, zeros past the end.
+  auto fetch = [&](int i) {
+    const int key0 = first + (warp + i * W) * kStep;
+    if (key0 < end) {
+      const uint32_t dst = ring + (i % Mem::kRing) * Mem::kBytes;
+      const bool whole = key0 + kStep <= end;
+      constexpr int kKeys = 32 / Mem::kChunks;  // keys of one round of the warp: 8 (8-bit kinds) or 4
+#pragma unroll
+      for (int n = 0; n < kStep / kKeys; ++n) {
+        const int at = (key0 + n * kKeys) & ((1 << sh) - 1);  // (a round lies inside one page)
+        const unsigned long long off = (unsigned long long)page_of(key0 + n * kKeys) * (page_vecs * Mem::kRow) +
+                                       (uint32_t)(at * Mem::kRow);
+        const int kk = n * kKeys + lane / Mem::kChunks, ch = lane % Mem::kChunks;
+        const bool live = whole || key0 + kk < end;
+        cp_async_or_zero16(dst + Mem::k_at(kk, ch), k0 + off, live);
+        cp_async_or_zero16(dst + Mem::v_at(kk, ch), v0 + off, live);
+      }
+      if constexpr (Mem::kQ8) {
+        const unsigned long long at = (unsigned long long)page_of(key0 + lane) * page_vecs + ((uint32_t)kvh << sh) +
+                                      ((key0 + lane) & ((1 << sh) - 1));
+        const bool live = whole || key0 + lane < end;
+        cp_async_or_zero4(dst + Mem::kScale + lane * 4, a.c.k_scale + at, live);
+        cp_async_or_zero4(dst + Mem::kScale + (kStep + lane) * 4, a.c.v_scale + at, live);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < Mem::kRing; ++i) fetch(i);
+  for (int i = 0;; ++i) {
+    const int key0 = first + (warp + i * W) * kStep;
+    if (key0 >= end) break;
+    cp_async_wait<Mem::kRing - 1>();
+    __syncwarp();
+    const uint32_t src = ring + (i % Mem::kRing) * Mem::kBytes;
     // S = Q·Kᵀ
     float s[MT][4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t kb[8];
       if constexpr (KIND == B2P_KV_16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) kb[i] = cur.k[j][i];
+        const uint4 x = lds16(src + Mem::k_at(8 * j + g, 2 * t)), y = lds16(src + Mem::k_at(8 * j + g, 2 * t + 1));
+        kb[0] = x.x, kb[1] = x.y, kb[2] = x.z, kb[3] = x.w, kb[4] = y.x, kb[5] = y.y, kb[6] = y.z, kb[7] = y.w;
       } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) widen4<T, KIND>(cur.k[j][i], kb[2 * i], kb[2 * i + 1]);
+        const uint4 x = lds16(src + Mem::k_at(8 * j + g, t));
+        widen4<T, KIND>(x.x, kb[0], kb[1]);
+        widen4<T, KIND>(x.y, kb[2], kb[3]);
+        widen4<T, KIND>(x.z, kb[4], kb[5]);
+        widen4<T, KIND>(x.w, kb[6], kb[7]);
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         s[m][j][0] = s[m][j][1] = s[m][j][2] = s[m][j][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t qa[4] = {q[m][0][2 * k], q[m][1][2 * k], q[m][0][2 * k + 1], q[m][1][2 * k + 1]};
-          mma16816<T>(s[m][j], qa, kb[2 * k], kb[2 * k + 1]);
-        }
+        for (int k = 0; k < 4; ++k) mma16816<T>(s[m][j], q[m][k], kb[2 * k], kb[2 * k + 1]);
       }
     }
-    // V of the step as B fragments: pair (key 2t, key 2t + 1) of tile j, channel 8g + n
-    uint32_t vb[4][8];
+    // scores in the log2 domain, masked where a row's keys end; the value's scale joins in
+    const bool whole = key0 + kStep <= min_lim;
+    float vi[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint32_t w[2][4];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if constexpr (KIND == B2P_KV_16) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[e][i] = cur.v[j][e][i];
-        } else {
-          widen4<T, KIND>(cur.v[j][e][0], w[e][0], w[e][1]);
-          widen4<T, KIND>(cur.v[j][e][1], w[e][2], w[e][3]);
-        }
+      float kc[2] = {kScaleLog2, kScaleLog2}, vl[2] = {0.f, 0.f};
+      if constexpr (KIND != B2P_KV_16) {
+        const uint2 ks = lds8(src + Mem::kScale + (8 * j + 2 * t) * 4);
+        const uint2 vs = lds8(src + Mem::kScale + (kStep + 8 * j + 2 * t) * 4);
+        // (a key that is not there has scale 0: its weight is 0, and 1 in the place of 1 / 0)
+        const float v0 = vs.x ? __uint_as_float(vs.x) : 1.f, v1 = vs.y ? __uint_as_float(vs.y) : 1.f;
+        kc[0] = __uint_as_float(ks.x) * kScaleLog2;
+        kc[1] = __uint_as_float(ks.y) * kScaleLog2;
+        vl[0] = log2_sfu(v0);
+        vl[1] = log2_sfu(v1);
+        vi[j][0] = rcp_sfu(v0);
+        vi[j][1] = rcp_sfu(v1);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vb[j][2 * i] = __byte_perm(w[0][i], w[1][i], 0x5410);
-        vb[j][2 * i + 1] = __byte_perm(w[0][i], w[1][i], 0x7632);
-      }
-    }
-    float kc[4][2], vl[4][2], vi[4][2];  // per key: factor of S, log2 of the value's scale, its inverse
-    if constexpr (KIND != B2P_KV_16) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        kc[j][0] = cur.ks[j].x * kScaleLog2;
-        kc[j][1] = cur.ks[j].y * kScaleLog2;
-        vl[j][0] = log2_sfu(cur.vs[j].x);
-        vl[j][1] = log2_sfu(cur.vs[j].y);
-        vi[j][0] = __frcp_rn(cur.vs[j].x);
-        vi[j][1] = __frcp_rn(cur.vs[j].y);
-      }
-    }
-    const int next = key0 + kRowWarps * kStep;
-    if (next < end) load_step<KIND>(cur, a.c, s_pages, first, kvh, next, end, g, t);
-
-    // scores in the log2 domain, masked where a row's keys end
-    const bool whole = key0 + kStep <= min_lim;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s[m][j][i] = KIND == B2P_KV_16 ? s[m][j][i] * kScaleLog2 : fmaf(s[m][j][i], kc[j][i & 1], vl[j][i & 1]);
+          s[m][j][i] = KIND == B2P_KV_16 ? s[m][j][i] * kScaleLog2 : fmaf(s[m][j][i], kc[i & 1], vl[i & 1]);
         if (!whole) {
           const int key = key0 + 8 * j + 2 * t;
 #pragma unroll
@@ -276,41 +338,89 @@ __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, in
           }
         }
       }
-      uint32_t pa[2][4];
+    }
+    // the rows' references move, to the next integer above, only for a score more than kSlack above them
+    bool up = false;
+    float top[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = -INFINITY;
+        float x = fmaxf(s[m][0][2 * e], s[m][0][2 * e + 1]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(s[m][j][2 * e], s[m][j][2 * e + 1]));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const float now = fmaxf(mx[m][e], top);
-        const float ref = now == -INFINITY ? 0.f : now;  // a row that sees none of the keys so far
-        const float scale = exp2_sfu(mx[m][e] - ref);
-        mx[m][e] = now;
+        for (int j = 1; j < 4; ++j) x = fmaxf(x, fmaxf(s[m][j][2 * e], s[m][j][2 * e + 1]));
+        top[m][e] = x;
+        up = up || x > mx[m][e] + kSlack;
+      }
+    if (__any_sync(~0u, up)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = top[m][e];
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+          const float now = x > mx[m][e] + kSlack ? ceilf(x) : mx[m][e];
+          const float f = now == mx[m][e] ? 1.f : exp2_sfu(mx[m][e] - now);
+          mx[m][e] = now;
+          l[m][e] *= f;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            o[m][n][2 * e] *= f;
+            o[m][n][2 * e + 1] *= f;
+          }
+        }
+    }
+    uint32_t pa[MT][2][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e];  // a row that sees none of the keys so far
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float p0 = exp2_sfu(s[m][j][2 * e] - ref), p1 = exp2_sfu(s[m][j][2 * e + 1] - ref);
           sum += KIND == B2P_KV_16 ? p0 + p1 : fmaf(p0, vi[j][0], p1 * vi[j][1]);
-          pa[j >> 1][(j & 1) * 2 + e] = pack_h2<T>(p0, p1);
+          pa[m][j >> 1][(j & 1) * 2 + e] = pack_h2<T>(p0, p1);
         }
-        l[m][e] = l[m][e] * scale + sum;
+        l[m][e] += sum;
+      }
+    // O += w·V: pairs (key 2t, key 2t + 1) of a tile, channel 8g + n
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          o[m][n][2 * e] *= scale;
-          o[m][n][2 * e + 1] *= scale;
+    for (int jj = 0; jj < 2; ++jj) {
+      uint32_t vb[2][8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = 8 * (2 * jj + j) + 2 * t;
+        if constexpr (KIND == B2P_KV_16) {
+          const uint4 x = lds16(src + Mem::v_at(key, g)), y = lds16(src + Mem::v_at(key + 1, g));
+          const uint32_t v[2][4] = {{x.x, x.y, x.z, x.w}, {y.x, y.y, y.z, y.w}};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            vb[j][2 * i] = __byte_perm(v[0][i], v[1][i], 0x5410);
+            vb[j][2 * i + 1] = __byte_perm(v[0][i], v[1][i], 0x7632);
+          }
+        } else {
+          const uint2 x = lds8(src + Mem::v_at(key, g >> 1) + (g & 1) * 8);
+          const uint2 y = lds8(src + Mem::v_at(key + 1, g >> 1) + (g & 1) * 8);
+          widen4<T, KIND>(__byte_perm(x.x, y.x, 0x5140), vb[j][0], vb[j][1]);
+          widen4<T, KIND>(__byte_perm(x.x, y.x, 0x7362), vb[j][2], vb[j][3]);
+          widen4<T, KIND>(__byte_perm(x.y, y.y, 0x5140), vb[j][4], vb[j][5]);
+          widen4<T, KIND>(__byte_perm(x.y, y.y, 0x7362), vb[j][6], vb[j][7]);
         }
       }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        mma16816<T>(o[m][n], pa[0], vb[0][n], vb[1][n]);
-        mma16816<T>(o[m][n], pa[1], vb[2][n], vb[3][n]);
-      }
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) mma16816<T>(o[m][n], pa[m][jj], vb[0][n], vb[1][n]);
     }
+    __syncwarp();
+    fetch(i + Mem::kRing);
   }
 
-  // join the warps' parts
+  const int count = row_end - row0;
+  const long long at0 = ((long long)part * a.c.kv_heads + kvh) * a.rows + row0;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -319,74 +429,84 @@ __global__ void __launch_bounds__(kRowThreads) attn_rows_kernel(PrefixArgs a, in
       sum += __shfl_xor_sync(~0u, sum, 1);
       sum += __shfl_xor_sync(~0u, sum, 2);
       const int r = m * 16 + e * 8 + g;
-      if (t == 0) s_ml[warp][r] = make_float2(mx[m][e], sum);
+      if (r < count) {
+        if (t == 0) (W == 1 ? a.part_ml[at0 + r] : s_ml[warp][r]) = make_float2(mx[m][e], sum);
+        float* dst = (W == 1 ? a.part_o + (at0 + r) * kKvHeadDim : &s_o[warp][r][0]) + 16 * t;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        s_o[warp][r][16 * t + n] = o[m][n][2 * e];
-        s_o[warp][r][16 * t + 8 + n] = o[m][n][2 * e + 1];
+        for (int n = 0; n < 8; n += 4) {
+          *reinterpret_cast<float4*>(dst + n) =
+              make_float4(o[m][n][2 * e], o[m][n + 1][2 * e], o[m][n + 2][2 * e], o[m][n + 3][2 * e]);
+          *reinterpret_cast<float4*>(dst + 8 + n) =
+              make_float4(o[m][n][2 * e + 1], o[m][n + 1][2 * e + 1], o[m][n + 2][2 * e + 1], o[m][n + 3][2 * e + 1]);
+        }
       }
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < MT * 16 * 16; i += kRowThreads) {
-    const int r = i >> 4, d = (i & 15) * 4;
-    if (row0 + r >= row_end) continue;
-    float top = -INFINITY;
+  if (W > 1) {  // join the warps' parts
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * 16; i += kRowThreads) {
+      const int r = i >> 4, d = (i & 15) * 4;
+      float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][r].x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-      const float f = exp2_sfu(s_ml[w][r].x - ref);
-      sum += f * s_ml[w][r].y;
-      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
-      acc.x += f * x.x;
-      acc.y += f * x.y;
-      acc.z += f * x.z;
-      acc.w += f * x.w;
+      for (int w = 0; w < W; ++w) {
+        const float f = exp2_sfu(s_ml[w][r].x - ref);
+        sum += f * s_ml[w][r].y;
+        const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
+        acc.x += f * x.x;
+        acc.y += f * x.y;
+        acc.z += f * x.z;
+        acc.w += f * x.w;
+      }
+      *reinterpret_cast<float4*>(a.part_o + (at0 + r) * kKvHeadDim + d) = acc;
+      if (d == 0) a.part_ml[at0 + r] = make_float2(top, sum);
     }
-    const long long at = ((long long)part * gridDim.y + kvh) * a.rows + row0 + r;
-    *reinterpret_cast<float4*>(a.part_o + at * kKvHeadDim + d) = acc;
-    if (d == 0) a.part_ml[at] = make_float2(top, sum);
   }
-  if (overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // and, with the last part of a row, all of them
+  if (FUSE) __threadfence();
+  if (!FUSE) {
+  } else if (W > 1) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kRowThreads) {
+      const int r = row0 + i;
+      if (shared && a.max_suffix > 0) len = suffix_len(a, r / span, status);
+      s_last[i] = row_complete(a, kvh, r, len) ? len : -1;
+    }
+    __syncthreads();
+    __threadfence();
+    for (int i = threadIdx.x >> 4; i < count; i += kRowThreads / 16)
+      if (s_last[i] >= 0) join_row<T>(a, kvh, row0 + i, s_last[i], threadIdx.x & 15);
+  } else {
+    __syncwarp();
+    if (shared && a.max_suffix > 0 && lane < count) len = suffix_len(a, (row0 + lane) / span, status);
+    const bool last = lane < count && row_complete(a, kvh, row0 + lane, len);
+    unsigned rows = __ballot_sync(~0u, last);
+    if (rows) __threadfence();
+    while (rows) {  // two at a time
+      const int r0 = __ffs(rows) - 1;
+      rows &= rows - 1;
+      const int r1 = rows ? __ffs(rows) - 1 : -1;
+      rows &= rows - 1;
+      const int r = lane < 16 ? r0 : r1;
+      const int n = __shfl_sync(~0u, len, r < 0 ? 0 : r);
+      if (r >= 0) join_row<T>(a, kvh, row0 + r, n, lane & 15);
+      __syncwarp();
+    }
+  }
+  if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// One half-warp per row: join the row's parts, normalise, round.
+// A half warp per row: join the row's parts (zeros where there is none).
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(PrefixArgs a, uint32_t* status) {
   pdl_enter();
-  const int heads_kv = gridDim.y, kvh = blockIdx.y;
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 4);
   if (r >= a.rows) return;
-  const int token = r / a.group;
-  const int len = a.max_suffix > 0 ? suffix_len(a, token / a.q_len, status) : 0;
-  const int used = a.max_suffix > 0 ? (len + a.suffix_chunk - 1) / a.suffix_chunk : 0;
-  const int shared = r < a.pair_rows ? a.n_prefix : a.n_last;
-  const int parts = shared + used;
-  auto part = [&](int p) { return p < shared ? p : p - shared + a.suffix_part; };
-  const long long stride = (long long)heads_kv * a.rows, at0 = (long long)kvh * a.rows + r;
-  float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[part(p) * stride + at0].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[part(p) * stride + at0];
-    const float f = exp2_sfu(ml.x - ref);
-    sum += f * ml.y;
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (part(p) * stride + at0) * kKvHeadDim + d);
-    acc.x += f * x.x;
-    acc.y += f * x.y;
-    acc.z += f * x.z;
-    acc.w += f * x.w;
-  }
-  const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-  const int h = kvh * a.group + r % a.group;
-  T* out = static_cast<T*>(a.out) + (long long)token * a.ld_out + h * kKvHeadDim + d;
-  *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2<T>(acc.x * inv, acc.y * inv), pack_h2<T>(acc.z * inv, acc.w * inv));
-  if (a.lse && d == 0) a.lse[(long long)token * heads_kv * a.group + h] = top == -INFINITY ? -INFINITY : ref + log2f(sum);
+  const int len = a.max_suffix > 0 ? suffix_len(a, r / (a.q_len * a.group), status) : 0;
+  join_row<T>(a, blockIdx.y, r, len, threadIdx.x & 15);
 }
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -395,6 +515,8 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 // longer than the page list that a block keeps.
 struct Plan {
   bool tc;  // the prefix goes to the tcgen05 kernel
+  int team;  // warps that share a unit of attn_rows_kernel
+  bool fuse; // whoever writes a row's last part joins the row; else attn_join_kernel does
   int mt, prefix_tiles, suffix_tiles, n_suffix, suffix_chunk;
   PrefixSplit split;
   int suffix_part, parts;
@@ -414,6 +536,7 @@ Plan make_plan(int batch, int q_len, int group, int kv_heads, int prefix_len, in
   p.mt = (p.tc || prefix_len == 0 ? q_len * group : rows) > 16 ? 2 : 1;
   p.prefix_tiles = ceil_div(rows, 16 * p.mt);
   p.suffix_tiles = ceil_div(q_len * group, 16 * p.mt);
+  p.team = kRowWarps;
   p.split.pair_rows = rows;
   if (p.tc) {
     prefix_tc_plan(rows, kv_heads, prefix_len, &p.split);
@@ -422,23 +545,45 @@ Plan make_plan(int batch, int q_len, int group, int kv_heads, int prefix_len, in
     p.split.n_prefix = ceil_div(prefix_len, p.split.prefix_chunk);
   }
   if (max_suffix > 0) {
-    p.suffix_chunk = chunk_for(max_suffix, batch * p.suffix_tiles * kv_heads, kWant);
+    const long long teams = (long long)batch * p.suffix_tiles * kv_heads;
+    p.suffix_chunk = chunk_for(max_suffix, (int)(teams < kWant ? teams : kWant), kWant);
+    if ((p.tc || prefix_len == 0) && teams >= kWant && max_suffix <= kTeamOneKeys) {
+      p.team = 1;
+      p.suffix_chunk = max_suffix <= kTeamOneKeys / 2 ? 128 : 256;
+    }
     p.n_suffix = ceil_div(max_suffix, p.suffix_chunk);
   }
   p.suffix_part = p.split.n_prefix > p.split.n_last ? p.split.n_prefix : p.split.n_last;
   p.parts = p.suffix_part + p.n_suffix;
+  p.fuse = !p.tc && p.parts > 0;
   return p;
 }
 
-template <typename T, int KIND, int MT>
+template <typename T, int KIND, int MT, int W, bool FUSE>
 int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   const long long prefix_units = p.tc ? 0 : (long long)p.split.n_prefix * p.prefix_tiles;
   const long long units = prefix_units + (long long)a.batch * p.n_suffix * p.suffix_tiles;
   B2P_REQUIRE(units < (1ll << 31), "too much work for one call");
-  B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT>, dim3((unsigned)units, a.c.kv_heads), dim3(kRowThreads), 0,
-                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, p.tc ? 1 : 0, c->status));
+  static thread_local uint64_t attr_mask = 0;  // one per instantiation
+  constexpr int kSmem = StepMem<KIND>::kBlock;
+  if (!(attr_mask & (1ull << (c->device & 63)))) {
+    B2P_CHECK_CUDA(cudaFuncSetAttribute(attn_rows_kernel<T, KIND, MT, W, FUSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kSmem));
+    attr_mask |= 1ull << (c->device & 63);
+  }
+  const int blocks = W == 1 ? ceil_div((int)units, kRowWarps) : (int)units;
+  B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT, W, FUSE>, dim3(blocks, a.c.kv_heads), dim3(kRowThreads), kSmem,
+                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, (int)units, c->status));
   B2P_POST_LAUNCH();
   return B2P_OK;
+}
+
+template <typename T, int KIND, bool FUSE>
+int launch_w(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
+  if (p.team == 1)
+    return p.mt == 2 ? launch_rows<T, KIND, 2, 1, FUSE>(a, p, c, st) : launch_rows<T, KIND, 1, 1, FUSE>(a, p, c, st);
+  return p.mt == 2 ? launch_rows<T, KIND, 2, kRowWarps, FUSE>(a, p, c, st)
+                   : launch_rows<T, KIND, 1, kRowWarps, FUSE>(a, p, c, st);
 }
 
 template <typename T, int KIND>
@@ -447,8 +592,8 @@ int run_t(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t s
   if (p.tc) rc = launch_prefix_tc(a, std::is_same<T, __nv_bfloat16>::value, st);
   if (rc) return rc;
   if (p.n_suffix > 0 || (p.split.n_prefix > 0 && !p.tc))
-    rc = p.mt == 2 ? launch_rows<T, KIND, 2>(a, p, c, st) : launch_rows<T, KIND, 1>(a, p, c, st);
-  if (rc) return rc;
+    rc = p.fuse ? launch_w<T, KIND, true>(a, p, c, st) : launch_w<T, KIND, false>(a, p, c, st);
+  if (rc || p.fuse) return rc;
   B2P_CHECK_CUDA(launch_pdl(attn_join_kernel<T>, dim3(ceil_div(a.rows, 8), a.c.kv_heads), dim3(128), 0, st, a,
                             c->status));
   B2P_POST_LAUNCH();
@@ -483,16 +628,17 @@ extern "C" {
 size_t b2p_attention_prefix_workspace(int batch, int q_len, int heads, int kv_heads, int prefix_len, int max_suffix) {
   if (!sizes_ok(batch, q_len, heads, kv_heads, prefix_len, max_suffix)) return 0;
   // A bound that grows with every argument, so that the workspace of the largest call serves all: parts are
-  // kTcStageKeys keys or longer, and there are about kWant blocks of 32 rows, or kSms of 256, or one per kMaxChunk keys.
+  // kTcStageKeys keys or longer, and there are about kWant blocks of 32 rows, or kSms of 256, or one per kMaxChunk keys,
+  // or at most 8 single-warp units a row.
   const long long rows = (long long)batch * q_len * heads;
   long long slots = 0;
   for (int len : {prefix_len, max_suffix}) {
     if (len == 0) continue;
     const long long by_length = rows * ceil_div(len, kTcStageKeys);
-    const long long by_blocks = (long long)kSms * 256 + rows * (2 + len / kMaxChunk);
+    const long long by_blocks = (long long)kSms * 256 + rows * (10 + len / kMaxChunk);
     slots += by_length < by_blocks ? by_length : by_blocks;
   }
-  return (size_t)slots * (kKvHeadDim * sizeof(float) + sizeof(float2)) + 256;
+  return (size_t)slots * (kKvHeadDim * sizeof(float) + sizeof(float2)) + (size_t)rows * sizeof(int) + 256;
 }
 
 int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, void* out, int ld_out, float* lse,
@@ -523,8 +669,11 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   B2P_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
   const int group = heads / a.c.kv_heads;
   const Plan p = make_plan(batch, q_len, group, a.c.kv_heads, prefix_len, max_suffix);
-  const size_t uses = (size_t)p.parts * batch * q_len * heads * (kKvHeadDim * 4 + sizeof(float2));
-  B2P_REQUIRE(uses <= workspace_bytes, "workspace bound of %zu bytes does not hold %zu", need, uses);
+  const size_t all_rows = (size_t)batch * q_len * heads;
+  const size_t uses = (size_t)p.parts * all_rows * (kKvHeadDim * sizeof(float) + sizeof(float2));
+  // the counts are at the end, where no call that shares the workspace keeps parts
+  const size_t counts = ((workspace_bytes & ~(size_t)15) - all_rows * sizeof(int)) & ~(size_t)15;
+  B2P_REQUIRE(uses <= counts, "workspace bound of %zu bytes does not hold %zu", need, uses);
   DeviceCtx* c = nullptr;
   if ((rc = ctx_get(&c))) return rc;
   a.q = q;
@@ -537,6 +686,7 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o +
                                         (size_t)p.parts * a.rows * a.c.kv_heads * kKvHeadDim);
+  a.arrived = reinterpret_cast<int*>(static_cast<char*>(workspace) + counts);
   a.ld_q = ld_q;
   a.ld_out = ld_out;
   a.batch = batch;
@@ -548,7 +698,7 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   static_cast<PrefixSplit&>(a) = p.split;
   a.suffix_part = p.suffix_part;
   a.n_suffix = p.n_suffix;
-  a.suffix_chunk = p.suffix_chunk;
+  a.suffix_chunk = p.suffix_chunk > 0 ? p.suffix_chunk : 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == B2P_BF16 ? run_kind<__nv_bfloat16>(a, p, c, st) : run_kind<__half>(a, p, c, st);
 }

@@ -8,7 +8,8 @@ namespace b2p {
 // Rows of one KV head: r = (b * q_len + i) * group + g, for query i of sequence b and query head
 // kvh * group + g. A part is what one kernel block computes for some rows over some keys: the rows'
 // maximum score (log2 domain), sum of exponentials and unnormalised output. The first parts split the
-// prefix, those from max(n_prefix, n_last) on each sequence's suffix, every split a fixed number of keys.
+// prefix, those from max(n_prefix, n_last) on each sequence's suffix, every split a fixed number of keys. For
+// few rows whoever writes the last part of a row joins them all; else attn_join_kernel does.
 struct PrefixSplit {
   int pair_rows;               // rows below it: n_prefix parts of prefix_chunk keys
   int n_prefix, prefix_chunk;
@@ -25,6 +26,7 @@ struct PrefixArgs : PrefixSplit {
   const int32_t* suffix_lens;
   float* part_o;    // [part][kv_heads * rows][64]
   float2* part_ml;  // [part][kv_heads * rows] (maximum, sum)
+  int* arrived;     // [kv_heads * rows] parts written so far; zero between calls
   long long ld_q, ld_out;
   int batch, q_len, group, rows;  // rows = batch * q_len * group, of one KV head
   int prefix_len, suffix_pitch, max_suffix;
@@ -48,6 +50,79 @@ __device__ __forceinline__ int suffix_len(const PrefixArgs& a, int b, uint32_t* 
     return 0;
   }
   return n;
+}
+
+// Parts of row r of a KV head, its suffix holding `len` tokens.
+__device__ __forceinline__ int parts_of(const PrefixArgs& a, int r, int len) {
+  return (r < a.pair_rows ? a.n_prefix : a.n_last) + (len + a.suffix_chunk - 1) / a.suffix_chunk;
+}
+
+__device__ __forceinline__ float exp2_sfu(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Join the parts of row r of KV head kvh and write the output, by the 16 threads of a half warp (sub = 0..15). The
+// order of the parts is fixed, whoever joins them.
+template <typename T>
+__device__ __forceinline__ void join_row(const PrefixArgs& a, int kvh, int r, int len, int sub) {
+  const unsigned half = 0xffffu << (threadIdx.x & 16);
+  const int shared = r < a.pair_rows ? a.n_prefix : a.n_last;
+  const int parts = parts_of(a, r, len);
+  const long long stride = (long long)a.c.kv_heads * a.rows, at0 = (long long)kvh * a.rows + r;
+  auto slot = [&](int p) { return (p < shared ? p : p - shared + a.suffix_part) * stride + at0; };
+  float top = -INFINITY;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += 16) {
+    if (p0 + sub < parts) {
+      ml = __ldcg(a.part_ml + slot(p0 + sub));
+      top = fmaxf(top, ml.x);
+    }
+  }
+  for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += 16) {
+    if (parts > 16) ml = p0 + sub < parts ? __ldcg(a.part_ml + slot(p0 + sub)) : make_float2(-INFINITY, 0.f);
+    const float f = exp2_sfu(ml.x - ref);
+    float part_sum = f * ml.y;
+    for (int o = 8; o; o >>= 1) part_sum += __shfl_xor_sync(half, part_sum, o);
+    sum += part_sum;
+    const int n = min(16, parts - p0);
+    for (int k0 = 0; k0 < n; k0 += 8) {  // eight loads in flight
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < n) x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(p0 + k0 + k) * kKvHeadDim) + sub);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(half, f, k0 + k, 16);
+        if (k0 + k < n) {
+          acc.x += w * x[k].x;
+          acc.y += w * x[k].y;
+          acc.z += w * x[k].z;
+          acc.w += w * x[k].w;
+        }
+      }
+    }
+  }
+  const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+  const int token = r / a.group, h = kvh * a.group + r % a.group;
+  T* out = static_cast<T*>(a.out) + (long long)token * a.ld_out + h * kKvHeadDim + sub * 4;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2<T>(acc.x * inv, acc.y * inv), pack_h2<T>(acc.z * inv, acc.w * inv));
+  if (a.lse && sub == 0)
+    a.lse[(long long)token * a.c.kv_heads * a.group + h] = top == -INFINITY ? -INFINITY : ref + log2f(sum);
+}
+
+// After a block has written a part of row r (threads of the block are past a fence and a barrier since): whether it
+// was the row's last. The one that finds so joins the row; the count is back at zero then.
+__device__ __forceinline__ bool row_complete(const PrefixArgs& a, int kvh, int r, int len) {
+  int* n = a.arrived + (long long)kvh * a.rows + r;
+  if (atomicAdd(n, 1) + 1 != parts_of(a, r, len)) return false;
+  *n = 0;
+  return true;
 }
 
 }  // namespace b2p

@@ -195,8 +195,10 @@ int b2p_kv_read(const b2p_kv_cache* cache, const int32_t* slots, int n_tokens, v
  * device; max_suffix bounds its entries and suffix_pitch >=
  * ceil(max_suffix/page_size). Query head h reads KV head h / (heads/kv_heads).
  * `workspace` holds at least b2p_attention_prefix_workspace() bytes (16-byte
- * aligned) for sizes that are at least this call's in each argument; calls that
- * share one must be ordered by their stream. Results repeat bit for bit. */
+ * aligned) for sizes that are at least this call's in each argument. It has to
+ * be zeroed once, before its first use and after a call that ended in a device
+ * error; calls that share one pass the same workspace_bytes and must be ordered
+ * by their stream. Results repeat bit for bit. */
 int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, void* out, int ld_out, float* lse,
                          int batch, int q_len, int heads, const int32_t* prefix_pages, int prefix_len,
                          const int32_t* suffix_pages, int suffix_pitch, const int32_t* suffix_lens, int max_suffix,
