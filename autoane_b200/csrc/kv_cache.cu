@@ -4,7 +4,10 @@
 // A vector of 64 channels (one token, one head) belongs to 8 lanes, 8 channels
 // each: one 16-byte load, the largest |x| by three shuffles, one 8-byte (codes)
 // or 16-byte store. The partner channels of a half-split rotation are in lane
-// +- rot/16 and come by shuffles of the 16-bit pairs as loaded.
+// +- rot/16 and come by shuffles of the 16-bit pairs as loaded. A warp has
+// four tokens and goes through their heads together, so that it need not diverge
+// between Q, K and V and loads a token's angles once.
+// Bound: the reads and writes (65536 tokens of 15 / 5 heads to int8: 380 MB).
 #include <cstdint>
 #include "decode.cuh"
 #include "ptx.cuh"
@@ -68,136 +71,152 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {  // a in the l
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
-
-template <typename T, int KIND, int HC>
-__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(AppendArgs a, uint32_t* status) {
-  pdl_enter();
-  const int total = a.heads + 2 * a.c.kv_heads;
-  const int chunks = (total + HC - 1) / HC;
-  const long long group = ((long long)blockIdx.x * kKvThreads + threadIdx.x) >> 3;
-  const int l = threadIdx.x & 7;
-  const bool live = group < (long long)a.n_tokens * chunks;
-  const int t = live ? (int)(group / chunks) : 0;
-  const int h0 = live ? (int)(group % chunks) * HC : 0;
-
-  const T* row = static_cast<const T*>(a.qkv) + (long long)t * a.ld_qkv;
-  uint4 raw[HC];
+// Four values of at most 127.5 as int8, rounded to nearest even: above 2^23 a sum's low byte is the integer.
+__device__ __forceinline__ uint32_t int8x4(const float* y) {
+  uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < HC; ++i)
-    raw[i] = (live && h0 + i < total) ? *reinterpret_cast<const uint4*>(row + (h0 + i) * kKvHeadDim + l * 8)
-                                      : make_uint4(0, 0, 0, 0);
-  int slot = -1;
-  if (live && h0 + HC > a.heads) {
-    slot = a.slots[t];
-    if (slot >= (a.c.n_pages << a.c.page_shift)) {
+  for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(__fadd_rn(y[i], 12582912.f));
+  return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+}
+
+enum RopeMode { ROPE_NONE, ROPE_HALVES, ROPE_PAIRS };
+
+// A warp takes every head of four tokens, four at a time with the next four on their way; or, where calls are small
+// (ONE), one head: the tokens' heads are then spread over more warps.
+template <typename T, int KIND, int MODE, bool ONE>
+__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(AppendArgs a, uint32_t* status) {
+  constexpr int HC = ONE ? 1 : 4;
+  pdl_enter();
+  const int kv = a.c.kv_heads, rotated = a.heads + kv, total = rotated + kv;
+  const int warp = (int)(((long long)blockIdx.x * kKvThreads + threadIdx.x) >> 5);
+  const int lane = threadIdx.x & 31, l = lane & 7;
+  const int first = ONE ? warp % total : 0, end = ONE ? first + 1 : total;
+  const int t = (ONE ? warp / total : warp) * 4 + (lane >> 3);
+  const bool live = t < a.n_tokens;
+
+  const T* row = static_cast<const T*>(a.qkv) + (live ? t : 0) * a.ld_qkv + l * 8;
+  auto load = [&](int h, uint4 (&raw)[HC]) {
+#pragma unroll
+    for (int i = 0; i < HC; ++i)
+      raw[i] = h + i < end ? __ldcs(reinterpret_cast<const uint4*>(row + (h + i) * kKvHeadDim)) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 raw[HC];
+  load(first, raw);
+  long long at0 = -1;  // vector of the token's slot, KV head 0
+  if (live && end > a.heads) {
+    const int slot = a.slots[t];
+    if (slot >= (a.c.n_pages << a.c.page_shift))
       atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
-      slot = -1;
-    }
+    else if (slot >= 0)
+      at0 = a.c.vec(slot >> a.c.page_shift, 0, slot & ((1 << a.c.page_shift) - 1));
   }
   // this lane's angles: channel j becomes x_j c_j + p_j s_j with p_j its partner channel, s_j negative for
-  // the first of a pair
+  // the first of a pair; outside the rotated part c = 1 and p = s = 0
   const bool turns = l * 8 < a.rot;
-  const int half_lanes = a.rot >> 4;  // lanes of one half of the rotated part
   float c[8], s[8];
-  if (a.rot && h0 < a.heads + a.c.kv_heads) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    c[e] = 1.f;
+    s[e] = 0.f;
+  }
+  int partner = lane;
+  if (MODE != ROPE_NONE && first < rotated) {
     int pos = live ? a.positions[t] : 0;
     if (pos < 0 || pos >= a.max_pos) {
-      if (live) atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
+      atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
       pos = 0;
     }
     const float4* tab = reinterpret_cast<const float4*>(a.rope + (long long)pos * a.rot);
-    if (turns) {
-      if (a.interleaved) {
+    if (turns && MODE == ROPE_PAIRS) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 w = __ldg(tab + l * 2 + i);
-          c[4 * i] = c[4 * i + 1] = w.x;
-          c[4 * i + 2] = c[4 * i + 3] = w.z;
-          s[4 * i] = -w.y;
-          s[4 * i + 1] = w.y;
-          s[4 * i + 2] = -w.w;
-          s[4 * i + 3] = w.w;
-        }
-      } else {
-        const bool second = l >= half_lanes;
-        const int l0 = second ? l - half_lanes : l;
+      for (int i = 0; i < 2; ++i) {
+        const float4 w = __ldg(tab + l * 2 + i);
+        c[4 * i] = c[4 * i + 1] = w.x;
+        c[4 * i + 2] = c[4 * i + 3] = w.z;
+        s[4 * i] = -w.y;
+        s[4 * i + 1] = w.y;
+        s[4 * i + 2] = -w.w;
+        s[4 * i + 3] = w.w;
+      }
+    } else if (turns) {
+      const int half_lanes = a.rot >> 4;  // lanes of one half of the rotated part
+      const bool second = l >= half_lanes;
+      partner = second ? lane - half_lanes : lane + half_lanes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 w = __ldg(tab + l0 * 4 + i);
-          c[2 * i] = w.x;
-          c[2 * i + 1] = w.z;
-          s[2 * i] = second ? w.y : -w.y;
-          s[2 * i + 1] = second ? w.w : -w.w;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float4 w = __ldg(tab + (second ? l - half_lanes : l) * 4 + i);
+        c[2 * i] = w.x;
+        c[2 * i + 1] = w.z;
+        s[2 * i] = second ? w.y : -w.y;
+        s[2 * i + 1] = second ? w.w : -w.w;
       }
     }
   }
-  const int lane = threadIdx.x & 31;
-  const int partner = !turns ? lane : a.interleaved ? lane : l >= half_lanes ? lane - half_lanes : lane + half_lanes;
 
+  T* q_out = static_cast<T*>(a.q_out) + (live ? t : 0) * a.ld_q + l * 8;
+#pragma unroll 1
+  for (int h0 = first; h0 < end; h0 += HC) {
+    uint4 next[HC];
+    if (!ONE) load(h0 + HC, next);
 #pragma unroll
-  for (int i = 0; i < HC; ++i) {
-    const int h = h0 + i;
-    uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&w[e]));
-      x[2 * e] = f.x;
-      x[2 * e + 1] = f.y;
-    }
-    if (a.rot) {  // every lane shuffles; a vector that does not turn keeps its channels
-      float p[8];
+    for (int i = 0; i < HC; ++i) {
+      const int h = h0 + i;  // (the same in all lanes)
+      if (h >= end) break;
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      float x[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        uint32_t o = __shfl_sync(~0u, w[e], partner);
-        const float2 f = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&o));
-        p[2 * e] = a.interleaved ? f.y : f.x;
-        p[2 * e + 1] = a.interleaved ? f.x : f.y;
+        const float2 f = H2<T>::to_f2(*reinterpret_cast<const typename H2<T>::V*>(&w[e]));
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
       }
-      if (turns && h < a.heads + a.c.kv_heads) {
+      if (MODE != ROPE_NONE && h < rotated) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + p[e] * s[e];
-      }
-    }
-    if (live && h < a.heads) {
-      T* q = static_cast<T*>(a.q_out) + (long long)t * a.ld_q + h * kKvHeadDim + l * 8;
-      *reinterpret_cast<uint4*>(q) = make_uint4(pack_h2<T>(x[0], x[1]), pack_h2<T>(x[2], x[3]), pack_h2<T>(x[4], x[5]),
-                                                pack_h2<T>(x[6], x[7]));
-    }
-    float top = 0.f;
-    if (KIND != B2P_KV_16) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(x[e]));
-      for (int o = 1; o < 8; o <<= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
-      top = max_nan(top, 1e-30f);
-    }
-    if (h < a.heads || h >= total || slot < 0) continue;
-    const bool is_v = h >= a.heads + a.c.kv_heads;
-    const int kvh = h - a.heads - (is_v ? a.c.kv_heads : 0);
-    const long long at = a.c.vec(slot >> a.c.page_shift, kvh, slot & ((1 << a.c.page_shift) - 1));
-    uint8_t* codes = is_v ? a.c.v : a.c.k;
-    if (KIND == B2P_KV_16) {
-      *reinterpret_cast<uint4*>(codes + at * 128 + l * 16) = make_uint4(
-          pack_h2<T>(x[0], x[1]), pack_h2<T>(x[2], x[3]), pack_h2<T>(x[4], x[5]), pack_h2<T>(x[6], x[7]));
-    } else {
-      constexpr float kTop = KIND == B2P_KV_INT8 ? 127.f : 448.f;
-      const float inv = __fmul_rn(__frcp_rn(top), kTop);
-      uint32_t o[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float* y = x + 4 * e;
-        if (KIND == B2P_KV_INT8) {
-          const int a0 = __float2int_rn(y[0] * inv), a1 = __float2int_rn(y[1] * inv);
-          const int a2 = __float2int_rn(y[2] * inv), a3 = __float2int_rn(y[3] * inv);
-          o[e] = (uint32_t)(a0 & 255) | (uint32_t)(a1 & 255) << 8 | (uint32_t)(a2 & 255) << 16 | (uint32_t)a3 << 24;
-        } else {
-          o[e] = e4m3_pair(y[0] * inv, y[1] * inv) | e4m3_pair(y[2] * inv, y[3] * inv) << 16;
+        for (int e = 0; e < 4; ++e) {
+          uint32_t o = MODE == ROPE_PAIRS ? __byte_perm(w[e], 0, 0x1032) : __shfl_sync(~0u, w[e], partner);
+          if (!turns) o = 0;
+          const float2 f = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&o));
+          x[2 * e] = x[2 * e] * c[2 * e] + f.x * s[2 * e];
+          x[2 * e + 1] = x[2 * e + 1] * c[2 * e + 1] + f.y * s[2 * e + 1];
         }
       }
-      *reinterpret_cast<uint2*>(codes + at * 64 + l * 8) = make_uint2(o[0], o[1]);
-      if (l == 0) (is_v ? a.c.v_scale : a.c.k_scale)[at] = top * (1.0f / kTop);
+      if (h < a.heads) {
+        if (live)
+          *reinterpret_cast<uint4*>(q_out + h * kKvHeadDim) = make_uint4(
+              pack_h2<T>(x[0], x[1]), pack_h2<T>(x[2], x[3]), pack_h2<T>(x[4], x[5]), pack_h2<T>(x[6], x[7]));
+        continue;
+      }
+      const bool is_v = h >= rotated;
+      const long long at = at0 + ((long long)(h - (is_v ? rotated : a.heads)) << a.c.page_shift);
+      uint8_t* codes = is_v ? a.c.v : a.c.k;
+      if (KIND == B2P_KV_16) {
+        if (at0 >= 0)
+          *reinterpret_cast<uint4*>(codes + at * 128 + l * 16) = make_uint4(
+              pack_h2<T>(x[0], x[1]), pack_h2<T>(x[2], x[3]), pack_h2<T>(x[4], x[5]), pack_h2<T>(x[6], x[7]));
+      } else {
+        float top = max_nan(fabsf(x[0]), fabsf(x[1]));
+#pragma unroll
+        for (int e = 2; e < 8; ++e) top = max_nan(top, fabsf(x[e]));
+        for (int o = 1; o < 8; o <<= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
+        top = max_nan(top, 1e-30f);
+        constexpr float kTop = KIND == B2P_KV_INT8 ? 127.f : 448.f;
+        const float inv = __fmul_rn(__frcp_rn(top), kTop);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], inv);
+        uint2 o;
+        if (KIND == B2P_KV_INT8)
+          o = make_uint2(int8x4(x), int8x4(x + 4));
+        else
+          o = make_uint2(e4m3_pair(x[0], x[1]) | e4m3_pair(x[2], x[3]) << 16,
+                         e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16);
+        if (at0 >= 0) {
+          *reinterpret_cast<uint2*>(codes + at * 64 + l * 8) = o;
+          if (l == 0) (is_v ? a.c.v_scale : a.c.k_scale)[at] = top * (1.0f / kTop);
+        }
+      }
     }
+#pragma unroll
+    for (int i = 0; i < HC; ++i) raw[i] = next[i];
   }
 }
 
@@ -210,65 +229,70 @@ struct ReadArgs {
   int n_tokens;
 };
 
+// K and V of one token and KV head by 8 lanes.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(ReadArgs a, uint32_t* status) {
   pdl_enter();
-  const int per = 2 * a.c.kv_heads;
   const long long group = ((long long)blockIdx.x * kKvThreads + threadIdx.x) >> 3;
   const int l = threadIdx.x & 7;
-  if (group >= (long long)a.n_tokens * per) return;
-  const int t = (int)(group / per);
-  const int h = (int)(group % per);
-  const bool is_v = h >= a.c.kv_heads;
-  const int kvh = is_v ? h - a.c.kv_heads : h;
+  if (group >= (long long)a.n_tokens * a.c.kv_heads) return;
+  const int t = (int)(group / a.c.kv_heads), kvh = (int)(group - (long long)t * a.c.kv_heads);
   int slot = a.slots[t];
   if (slot >= (a.c.n_pages << a.c.page_shift)) {
     atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
     slot = -1;
   }
-  uint4 r = make_uint4(0, 0, 0, 0);
+  uint4 r[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   if (slot >= 0) {
     const long long at = a.c.vec(slot >> a.c.page_shift, kvh, slot & ((1 << a.c.page_shift) - 1));
-    const uint8_t* codes = is_v ? a.c.v : a.c.k;
     if (KIND == B2P_KV_16) {
-      r = *reinterpret_cast<const uint4*>(codes + at * 128 + l * 16);
+      r[0] = *reinterpret_cast<const uint4*>(a.c.k + at * 128 + l * 16);
+      r[1] = *reinterpret_cast<const uint4*>(a.c.v + at * 128 + l * 16);
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(codes + at * 64 + l * 8);
-      const float scale = (is_v ? a.c.v_scale : a.c.k_scale)[at];
-      uint32_t p[4];
-      widen4<T, KIND>(w.x, p[0], p[1]);
-      widen4<T, KIND>(w.y, p[2], p[3]);
+      const uint2 w[2] = {*reinterpret_cast<const uint2*>(a.c.k + at * 64 + l * 8),
+                          *reinterpret_cast<const uint2*>(a.c.v + at * 64 + l * 8)};
+      const float scale[2] = {a.c.k_scale[at], a.c.v_scale[at]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&p[e]));
-        p[e] = pack_h2<T>(f.x * scale, f.y * scale);
+      for (int v = 0; v < 2; ++v) {
+        uint32_t p[4];
+        widen4<T, KIND>(w[v].x, p[0], p[1]);
+        widen4<T, KIND>(w[v].y, p[2], p[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&p[e]));
+          p[e] = pack_h2<T>(f.x * scale[v], f.y * scale[v]);
+        }
+        r[v] = make_uint4(p[0], p[1], p[2], p[3]);
       }
-      r = make_uint4(p[0], p[1], p[2], p[3]);
     }
   }
-  T* out = is_v ? static_cast<T*>(a.v_out) + (long long)t * a.ld_v : static_cast<T*>(a.k_out) + (long long)t * a.ld_k;
-  *reinterpret_cast<uint4*>(out + kvh * kKvHeadDim + l * 8) = r;
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (long long)t * a.ld_k + kvh * kKvHeadDim + l * 8) = r[0];
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.v_out) + (long long)t * a.ld_v + kvh * kKvHeadDim + l * 8) = r[1];
 }
 
-template <typename T, int KIND>
-int append_t(const AppendArgs& a, const DeviceCtx* c, cudaStream_t st) {
-  // One head per lane group while the call does not fill the GPU (latency), four heads of a token
-  // otherwise: a token's angles are then loaded once for four heads.
+template <typename T, int KIND, int MODE>
+int append_mode(const AppendArgs& a, const DeviceCtx* c, cudaStream_t st) {
+  // One head a warp while that does not fill the GPU four times over: a warp that goes through 25 heads takes longer
+  // than the whole call of a few tokens.
   const int total = a.heads + 2 * a.c.kv_heads;
-  const bool few = (long long)a.n_tokens * total * 8 <= (long long)c->num_sms * 2048;
-  const int hc = few ? 1 : 4;
-  const long long threads = (long long)a.n_tokens * ((total + hc - 1) / hc) * 8;
-  const long long blocks = (threads + kKvThreads - 1) / kKvThreads;
-  B2P_REQUIRE(blocks < (1ll << 31), "too many tokens in one call");
-  B2P_CHECK_CUDA(launch_pdl(few ? kv_append_kernel<T, KIND, 1> : kv_append_kernel<T, KIND, 4>, dim3((unsigned)blocks),
-                            dim3(kKvThreads), 0, st, a, c->status));
+  const long long quads = ((long long)a.n_tokens + 3) / 4;
+  const bool one = quads * total <= (long long)c->num_sms * 64 * 4;
+  const long long blocks = (quads * (one ? total : 1) * 32 + kKvThreads - 1) / kKvThreads;
+  B2P_CHECK_CUDA(launch_pdl(one ? kv_append_kernel<T, KIND, MODE, true> : kv_append_kernel<T, KIND, MODE, false>,
+                            dim3((unsigned)blocks), dim3(kKvThreads), 0, st, a, c->status));
   B2P_POST_LAUNCH();
   return B2P_OK;
 }
 
 template <typename T, int KIND>
+int append_t(const AppendArgs& a, const DeviceCtx* c, cudaStream_t st) {
+  if (!a.rot) return append_mode<T, KIND, ROPE_NONE>(a, c, st);
+  return a.interleaved ? append_mode<T, KIND, ROPE_PAIRS>(a, c, st) : append_mode<T, KIND, ROPE_HALVES>(a, c, st);
+}
+
+template <typename T, int KIND>
 int read_t(const ReadArgs& a, const DeviceCtx* c, cudaStream_t st) {
-  const long long threads = (long long)a.n_tokens * 2 * a.c.kv_heads * 8;
+  const long long threads = (long long)a.n_tokens * a.c.kv_heads * 8;
   const long long blocks = (threads + kKvThreads - 1) / kKvThreads;
   B2P_REQUIRE(blocks < (1ll << 31), "too many tokens in one call");
   B2P_CHECK_CUDA(

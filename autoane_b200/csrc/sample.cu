@@ -63,12 +63,15 @@ struct Params {
   int k;             // 0: off
   float p;           // 1: off
   uint32_t least;    // min-p as a weight
+  float u;
 };
 
-__device__ __forceinline__ Params params_of(const SampleArgs& a, int r, float m) {
+// (all but the maximum, which is not known yet when they are read)
+__device__ __forceinline__ Params params_of(const SampleArgs& a, int r) {
   Params q;
   const float t = a.temperature ? a.temperature[r] : 1.f;
-  q.m = m;
+  q.m = 0.f;
+  q.u = a.u[r];
   q.cold = !(t > 0.f);
   q.c = q.cold ? 0.f : __fmul_rn(__frcp_rn(t), 1.4426950408889634f) * kSteps;
   const int k = a.top_k ? a.top_k[r] : 0;
@@ -113,7 +116,7 @@ struct Found {  // a bin, and the sums before it
 template <int NT>
 struct Scan {
   u64 c[NT / 32], w[NT / 32];
-  Found found;
+  Found found[3];  // bin kBins before each use
 };
 
 // A histogram's running sums: each thread has those before its kBins / NT bins.
@@ -147,24 +150,20 @@ __device__ __forceinline__ void scan_bins(Scan<NT>& s, const uint32_t* count, co
     w += s.w[k];
   }
 }
-// The first bin at which the measure (counts, or weights) reaches `aim` (> 0); bin kBins if none. c, w: scan_bins' sums.
+// The first bin at which the measure (counts, or weights) reaches `aim` (> 0), into found[slot] after the next barrier;
+// c, w: scan_bins' sums.
 template <int NT>
-__device__ __forceinline__ Found find_bin(Scan<NT>& s, const uint32_t* count, const u64* weight, u64 c, u64 w,
-                                          bool by_count, u64 aim) {
+__device__ __forceinline__ void find_bin(Scan<NT>& s, const uint32_t* count, const u64* weight, u64 c, u64 w,
+                                         bool by_count, u64 aim, int slot) {
   constexpr int kEach = kBins / NT;
-  __syncthreads();
-  if (threadIdx.x == 0) s.found = {kBins, 0, 0};
-  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int b = threadIdx.x * kEach + i;
     const u64 nc = c + count[b], nw = w + weight[b];
-    if (nc > c && (by_count ? c : w) < aim && (by_count ? nc : nw) >= aim) s.found = {b, c, w};  // one bin at most
+    if (nc > c && (by_count ? c : w) < aim && (by_count ? nc : nw) >= aim) s.found[slot] = {b, c, w};  // one bin at most
     c = nc;
     w = nw;
   }
-  __syncthreads();
-  return s.found;
 }
 
 // top-p's aim as an integer: sums below it are below p of `kept`.
@@ -236,7 +235,11 @@ __device__ Cut long_cut(LongMem<NT>& s, const T* x, int vocab, const Params& q, 
     long_histogram<NT, T>(s, x, vocab, q, prefix, above, above == 5 ? 5 : 10);
     u64 c, w;
     scan_bins<NT>(s.scan, s.count, s.weight, c, w);
-    const Found f = find_bin<NT>(s.scan, s.count, s.weight, c + c0, w + w0, by_count, aim);
+    if (threadIdx.x == 0) s.scan.found[0] = {kBins, 0, 0};
+    __syncthreads();
+    find_bin<NT>(s.scan, s.count, s.weight, c + c0, w + w0, by_count, aim, 0);
+    __syncthreads();
+    const Found f = s.scan.found[0];
     if (f.bin == kBins) {  // (on the first level only)
       kept = 0;
       for (int i = 0; i < NT / 32; ++i) kept += s.scan.w[i];
@@ -339,7 +342,7 @@ __device__ __noinline__ void long_row(LongMem<NT>& s, const SampleArgs& a, int r
     if (i == warp) run = total;
     total += s.n[i];
   }
-  const u64 aim = aim_of(a.u[r], total);
+  const u64 aim = aim_of(q.u, total);
   if (run <= aim && aim < run + w) walk(a, r, x, q, lo, hi, cut, run, aim, total);
 }
 
@@ -360,7 +363,9 @@ __global__ void __launch_bounds__(kLongThreads) sample_long_kernel(SampleArgs a)
     if (threadIdx.x == 0) put_none(a, r);
     return;
   }
-  long_row<kLongThreads, T>(s, a, r, x, params_of(a, r, m));
+  Params q = params_of(a, r);
+  q.m = m;
+  long_row<kLongThreads, T>(s, a, r, x, q);
 }
 
 // ---------------------------------------------------------------------------
@@ -489,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
   const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0;
   const int r = blockIdx.x / ctas;
   const T* row = static_cast<const T*>(a.logits) + (long long)r * a.ld;
+  Params q = params_of(a, r);
   // A CTA's slice goes by 16-byte vectors, so the row begins `skew` places into the first one. Index order is that of
   // (rank, warp, load, lane, place in the vector).
   const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
@@ -507,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
       for (int k = 0; k < kVec; ++k) x[i * kVec + k] = j + k >= 0 && j + k < a.vocab ? to_float(row[j + k]) : -INFINITY;
     }
   }
+  if (threadIdx.x < 3) s.scan.found[threadIdx.x] = {kBins, 0, 0};
   if (threadIdx.x == 0) s.listed = 0;
   // the row's maximum
   float m = x[0];
@@ -527,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
     if (rank == 0 && threadIdx.x == 0) put_none(a, r);
     return;
   }
-  const Params q = params_of(a, r, m);
+  q.m = m;
   if (q.cold || m == INFINITY) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = x[i] == m ? 0.f : INFINITY;
@@ -582,16 +589,23 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
     if (rank == 0) {
       u64 c, w;
       scan_bins<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w);
-      if (k) fk = find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, true, (u64)k);
+      if (k) {
+        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, true, (u64)k, 0);
+        __syncthreads();
+        fk = s.scan.found[0];
+      }
       int lo = kBins, hi = -1;
       if (by_p) {
         for (int i = 0; i < kWarps; ++i) all_w += s.scan.w[i];
         const u64 least_w = fk.bin < kBins ? fk.weight : all_w;
         const u64 most_w = fk.bin < kBins ? fk.weight + s.h.all_weight[fk.bin] : all_w;
         const u64 lo_aim = max(p_aim(q.p, least_w), (u64)1), hi_aim = max(p_aim(q.p, most_w), (u64)1);
-        fp = find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, lo_aim);
-        lo = hi = fp.bin;
-        if (hi_aim > lo_aim) hi = find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, hi_aim).bin;
+        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, lo_aim, 1);
+        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, hi_aim, 2);
+        __syncthreads();
+        fp = s.scan.found[1];
+        lo = fp.bin;
+        hi = s.scan.found[2].bin;
       }
       if (threadIdx.x < ctas) {
         *remote(&s.lo_bin, threadIdx.x) = lo;
@@ -601,18 +615,35 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
     }
     sync();
     if (s.k_bin < kBins || s.lo_bin < kBins) {
+      // (keys up to kLive only: a bin that is none begins there)
       const float lo_key = (float)(s.lo_bin << 15), hi_key = (float)((s.hi_bin + 1) << 15);
-      const float k_lo = (float)(s.k_bin << 15), k_hi = (float)((s.k_bin + 1) << 15);
+      const float k_lo = (float)(s.k_bin << 15), k_hi = s.k_bin < kBins ? (float)((s.k_bin + 1) << 15) : k_lo;
       uint32_t* const listed = remote(&s.listed, 0);
       u64* const list = remote(&s.list[0], 0);
       uint32_t* const list_w = remote(&s.list_w[0], 0);
+      // (one atomic of each warp on the first CTA's count: a round trip takes about a thousand cycles)
+      uint32_t mine = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (x[i] < kLive && ((x[i] >= lo_key && x[i] < hi_key) || (x[i] >= k_lo && x[i] < k_hi))) {
-          const uint32_t at = atomicAdd(listed, 1u);
-          if (at < kList) {
-            list[at] = token_of((uint32_t)x[i], first + (i / kVec) * 32 * kVec + i % kVec);
-            list_w[at] = weight_of(x[i]);
+      for (int i = 0; i < kPer; ++i)
+        mine |= (uint32_t)((x[i] >= lo_key && x[i] < hi_key) || (x[i] >= k_lo && x[i] < k_hi)) << i;
+      const uint32_t n = __popc(mine);
+      uint32_t at = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t p = __shfl_up_sync(~0u, at, o);
+        if (lane >= o) at += p;
+      }
+      uint32_t from = 0;
+      if (lane == 31 && at) from = atomicAdd(listed, at);
+      at += __shfl_sync(~0u, from, 31) - n;
+      if (__any_sync(~0u, n != 0)) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (mine >> i & 1) {
+            if (at < kList) {
+              list[at] = token_of((uint32_t)x[i], first + (i / kVec) * 32 * kVec + i % kVec);
+              list_w[at] = weight_of(x[i]);
+            }
+            at += 1;
           }
         }
       }
@@ -647,7 +678,15 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
     for (int i = 0; i < kPer; ++i) w += weight_of(x[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) w += kept(i);
+    for (int i = 0; i < kPer; i += kVec) {  // (most loads of a row that is cut hold no token that stays)
+      float least_key = x[i];
+#pragma unroll
+      for (int k = 1; k < kVec; ++k) least_key = fminf(least_key, x[i + k]);
+      if (__any_sync(~0u, least_key <= cut_key)) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) w += kept(i + k);
+      }
+    }
   }
   w = warp_sum(w);
   __syncthreads();
@@ -667,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int c
       total += s.w[i];
     }
   }
-  const u64 aim = aim_of(a.u[r], total);
+  const u64 aim = aim_of(q.u, total);
   if (aim < run || aim >= run + w) return;
   // the warp that has it: the load, then the lane, then the token at which the running sum passes the aim
   uint32_t y[kVec];
