@@ -33,31 +33,36 @@ _LOGITS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _KIND = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3, torch.float16: KV_16, torch.bfloat16: KV_16}
 
 
+_bound: dict = {}
+
+
 def _fn(name):
-    """The entry point, without argtypes conversion beyond ctypes' own."""
-    return getattr(_lib.load(), name)
+    """The library's entry point."""
+    f = _bound.get(name)
+    if f is None:
+        f = _bound[name] = getattr(_lib.load(), name)
+    return f
 
 
 def _raise(name: str, rc: int):
     raise B2PError(name, rc, _lib.load().b2p_last_error().decode(errors="replace"))
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index
 
 
 def _rows(t: torch.Tensor, name: str, dtypes=_DTYPE) -> torch.Tensor:
-    if t.dim() != 2 or t.dtype not in dtypes or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dim() != 2 or t.dtype not in dtypes or not t.is_cuda or (t.stride(1) != 1 and t.shape[1] > 1):
         raise ValueError(f"{name} must be a CUDA matrix of {[str(d) for d in dtypes]} with contiguous rows")
     return t
 
 
-def _vec(t, name: str, dtype, n: int, device):
+def _vec(t, name: str, dtype, n: int, device: int):
     """A contiguous vector's address; None gives NULL."""
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on {device}")
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on cuda:{device}")
     return t.data_ptr()
 
 
@@ -120,7 +125,7 @@ class KVCache:
         self.k, self.v = k, v
         self.k_scale, self.v_scale = scales or (None, None)
         self.n_pages, self.kv_heads, self.page_size, _ = k.shape
-        self.kind, self.device = kind, k.device
+        self.kind, self.device, self._dev = kind, k.device, k.get_device()
         self._desc = KVCacheDesc(k.data_ptr(), v.data_ptr(), *(s.data_ptr() for s in scales or ()),
                                  *((None, None) if not scales else ()), self.n_pages, self.page_size, self.kv_heads,
                                  kind)
@@ -146,23 +151,28 @@ class KVCache:
         """Write the K and V of qkv [n, 64·(heads + 2·kv_heads)] to `slots` (int32 [n]; negative: skip), rotated by
         `table` (see rope_table; None: no rotation) at `positions` (int32 [n]). Returns rotated Q [n, 64·heads]
         (`out`, which may be a view of qkv)."""
-        _rows(qkv, "qkv")
-        n = qkv.shape[0]
-        if qkv.shape[1] < HEAD_DIM * (heads + 2 * self.kv_heads) or qkv.device != self.device:
-            raise ValueError(f"qkv must have {HEAD_DIM * (heads + 2 * self.kv_heads)} columns, on {self.device}")
+        n, cols = _rows(qkv, "qkv").shape
+        q_cols, dev = heads * HEAD_DIM, self._dev
+        if cols < q_cols + 2 * HEAD_DIM * self.kv_heads or qkv.get_device() != dev:
+            raise ValueError(f"qkv must have {q_cols + 2 * HEAD_DIM * self.kv_heads} columns, on {self.device}")
         if out is None:
-            out = torch.empty((n, heads * HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
-        elif out.shape != (n, heads * HEAD_DIM) or out.dtype != qkv.dtype or out.device != qkv.device:
-            raise ValueError(f"out must be {qkv.dtype} [{n}, {heads * HEAD_DIM}] on {qkv.device}")
-        if table is not None and (table.dim() != 3 or table.shape[2] != 2 or positions is None):
-            raise ValueError("table must be [positions, rot/2, 2], and goes with positions")
-        max_pos, rot = (table.shape[0], 2 * table.shape[1]) if table is not None else (0, 0)
+            out = qkv.new_empty((n, q_cols))
+            ld_out = q_cols
+        else:
+            if out.shape != (n, q_cols) or out.dtype is not qkv.dtype or out.get_device() != dev:
+                raise ValueError(f"out must be {qkv.dtype} [{n}, {q_cols}] on {self.device}")
+            ld_out = _ld(_rows(out, "out"))
+        max_pos = rot = 0
+        angles = None
+        if table is not None:
+            if table.dim() != 3 or table.shape[2] != 2 or positions is None:
+                raise ValueError("table must be [positions, rot/2, 2], and goes with positions")
+            max_pos, rot = table.shape[0], 2 * table.shape[1]
+            angles = _vec(table, "table", torch.float32, max_pos * rot, dev)
         rc = _fn("b2p_kv_append")(
-            self._ref, qkv.data_ptr(), _ld(qkv), heads, _rows(out, "out").data_ptr(), _ld(out),
-            _vec(slots, "slots", torch.int32, n, self.device),
-            _vec(positions, "positions", torch.int32, n, self.device),
-            None if table is None else _vec(table, "table", torch.float32, max_pos * rot, self.device),
-            max_pos, rot, int(interleaved), n, self._dtype(qkv.dtype), _stream(qkv))
+            self._ref, qkv.data_ptr(), _ld(qkv), heads, out.data_ptr(), ld_out,
+            _vec(slots, "slots", torch.int32, n, dev), _vec(positions, "positions", torch.int32, n, dev), angles,
+            max_pos, rot, 1 if interleaved else 0, n, self._dtype(qkv.dtype), _stream(dev))
         if rc:
             _raise("b2p_kv_append", rc)
         return out
@@ -170,17 +180,16 @@ class KVCache:
     def read(self, slots: torch.Tensor, dtype: torch.dtype, k_out: torch.Tensor | None = None,
              v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The K and V of `slots` (int32 [n]; negative: zeros) as [n, 64·kv_heads] of `dtype`."""
-        n, cols = slots.numel(), HEAD_DIM * self.kv_heads
-        outs = []
+        n, cols, dev = slots.numel(), HEAD_DIM * self.kv_heads, self._dev
+        code = self._dtype(dtype)
         for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is None:
-                t = torch.empty((n, cols), dtype=dtype, device=self.device)
-            elif t.shape != (n, cols) or t.dtype != dtype or t.device != self.device:
+            if t is not None and (t.shape != (n, cols) or t.dtype is not dtype or t.get_device() != dev):
                 raise ValueError(f"{name} must be {dtype} [{n}, {cols}] on {self.device}")
-            outs.append(_rows(t, name))
-        k, v = outs
-        rc = _fn("b2p_kv_read")(self._ref, _vec(slots, "slots", torch.int32, n, self.device), n, k.data_ptr(), _ld(k),
-                                v.data_ptr(), _ld(v), self._dtype(dtype), _stream(slots))
+        k = torch.empty((n, cols), dtype=dtype, device=self.device) if k_out is None else _rows(k_out, "k_out")
+        v = torch.empty_like(k) if v_out is None else _rows(v_out, "v_out")
+        rc = _fn("b2p_kv_read")(self._ref, _vec(slots, "slots", torch.int32, n, dev), n, k.data_ptr(),
+                                cols if k_out is None else _ld(k), v.data_ptr(), cols if v_out is None else _ld(v),
+                                code, _stream(dev))
         if rc:
             _raise("b2p_kv_read", rc)
         return k, v
@@ -199,41 +208,42 @@ class PrefixAttention:
         self.batch, self.q_len, self.heads, self.kv_heads = batch, q_len, heads, kv_heads
         self.max_prefix, self.max_suffix = max_prefix, max_suffix
         self.workspace = torch.zeros(size, dtype=torch.uint8, device=device)
+        self._ws, self._ws_bytes = self.workspace.data_ptr(), size
 
     def __call__(self, q: torch.Tensor, cache: KVCache, prefix_pages: torch.Tensor | None, prefix_len: int,
                  suffix_pages: torch.Tensor | None, suffix_lens: torch.Tensor | None, out: torch.Tensor | None = None,
                  return_lse: bool = False):
         """q [batch·q_len, 64·heads]; prefix_pages int32 [ceil(prefix_len/page_size)]; suffix_pages int32
         [batch, pages]; suffix_lens int32 [batch] (None: no suffixes). Returns out, or (out, lse [batch·q_len, heads])."""
-        n, dev = self.batch * self.q_len, cache.device
-        _rows(q, "q")
-        if q.shape != (n, self.heads * HEAD_DIM) or q.device != dev or cache.kv_heads != self.kv_heads:
-            raise ValueError(f"q must be [{n}, {self.heads * HEAD_DIM}] on {dev}, the cache have {self.kv_heads} KV heads")
+        n, cols, dev = self.batch * self.q_len, self.heads * HEAD_DIM, cache._dev
+        if _rows(q, "q").shape != (n, cols) or q.get_device() != dev or cache.kv_heads != self.kv_heads:
+            raise ValueError(f"q must be [{n}, {cols}] on {cache.device}, the cache have {self.kv_heads} KV heads")
         if not 0 <= prefix_len <= self.max_prefix:
             raise ValueError(f"prefix_len must be from 0 to {self.max_prefix}")
-        pages = -(-prefix_len // cache.page_size)
-        if prefix_len and (prefix_pages is None or prefix_pages.numel() < pages):
-            raise ValueError(f"prefix_pages must name {pages} pages")
-        most = self.max_suffix if suffix_lens is not None else 0
-        pitch = 0
-        if most:
+        prefix = pages = lens = None
+        pitch = most = 0
+        if prefix_len:
+            if prefix_pages is None or prefix_pages.numel() * cache.page_size < prefix_len:
+                raise ValueError(f"prefix_pages must name {-(-prefix_len // cache.page_size)} pages")
+            prefix = _vec(prefix_pages, "prefix_pages", torch.int32, prefix_pages.numel(), dev)
+        if suffix_lens is not None and self.max_suffix:
             if suffix_pages is None or suffix_pages.dim() != 2 or suffix_pages.shape[0] != self.batch:
                 raise ValueError("suffix_pages must be [batch, pages]")
             pitch = suffix_pages.shape[1]
-            most = min(most, pitch * cache.page_size)
+            most = min(self.max_suffix, pitch * cache.page_size)
+            if most:
+                pages = _vec(suffix_pages, "suffix_pages", torch.int32, self.batch * pitch, dev)
+                lens = _vec(suffix_lens, "suffix_lens", torch.int32, self.batch, dev)
+        ld_q = _ld(q)
         if out is None:
-            out = torch.empty((n, self.heads * HEAD_DIM), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            out = torch.empty_like(q) if ld_q == cols else q.new_empty((n, cols))
+        elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev:
             raise ValueError("out must be like q")
-        lse = torch.empty((n, self.heads), dtype=torch.float32, device=dev) if return_lse else None
-        i32 = torch.int32
+        lse = q.new_empty((n, self.heads), dtype=torch.float32) if return_lse else None
         rc = _fn("b2p_attention_prefix")(
-            cache._ref, q.data_ptr(), _ld(q), _rows(out, "out").data_ptr(), _ld(out),
-            None if lse is None else lse.data_ptr(), self.batch, self.q_len, self.heads,
-            _vec(prefix_pages, "prefix_pages", i32, prefix_pages.numel(), dev) if prefix_len else None, prefix_len,
-            _vec(suffix_pages, "suffix_pages", i32, self.batch * pitch, dev) if most else None, pitch,
-            _vec(suffix_lens, "suffix_lens", i32, self.batch, dev) if most else None, most,
-            cache._dtype(q.dtype), self.workspace.data_ptr(), self.workspace.numel(), _stream(q))
+            cache._ref, q.data_ptr(), ld_q, out.data_ptr(), _ld(_rows(out, "out")),
+            None if lse is None else lse.data_ptr(), self.batch, self.q_len, self.heads, prefix, prefix_len, pages,
+            pitch, lens, most, cache._dtype(q.dtype), self._ws, self._ws_bytes, _stream(dev))
         if rc:
             _raise("b2p_attention_prefix", rc)
         return (out, lse) if return_lse else out
@@ -245,19 +255,19 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
     """A token for each row of logits [n, vocab] (float16, bfloat16 or float32) from uniform numbers u (fp32 [n]),
     with per-row temperature, top_p, min_p (fp32 [n]) and top_k (int32 [n]); None turns a filter off. Returns tokens
     (int32 [n]; `out`) and the natural logs of their probabilities among the kept tokens (fp32 [n])."""
-    _rows(logits, "logits", _LOGITS)
-    n, dev = logits.shape[0], logits.device
-    if out is None:
-        out = torch.empty((n,), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((n,), dtype=torch.float32, device=dev)
-    f32, i32 = torch.float32, torch.int32
+    n, vocab = _rows(logits, "logits", _LOGITS).shape
+    dev = logits.get_device()
     if u is None:
         raise ValueError("u is needed")
+    logprobs = torch.empty_like(u)
+    f32, i32 = torch.float32, torch.int32
+    if out is None:
+        out = torch.empty_like(u, dtype=i32)
     rc = _fn("b2p_sample")(
-        logits.data_ptr(), _ld(logits), n, logits.shape[1], _LOGITS[logits.dtype], _vec(u, "u", f32, n, dev),
+        logits.data_ptr(), _ld(logits), n, vocab, _LOGITS[logits.dtype], _vec(u, "u", f32, n, dev),
         _vec(temperature, "temperature", f32, n, dev), _vec(top_k, "top_k", i32, n, dev),
         _vec(top_p, "top_p", f32, n, dev), _vec(min_p, "min_p", f32, n, dev), _vec(out, "out", i32, n, dev),
-        logprobs.data_ptr(), _stream(logits))
+        logprobs.data_ptr(), _stream(dev))
     if rc:
         _raise("b2p_sample", rc)
     return out, logprobs
