@@ -9,18 +9,23 @@
 // weights, both in a histogram of the upper key bits (1024 bins of 1/32 octave);
 // the tokens of the bins where the cuts lie are then gathered and ranked.
 //
-// sample_kernel: a cluster of up to 8 CTAs has a row, 8192 logits a CTA, 32 in
-// the registers of each thread, so that a row is read once. The CTAs exchange
-// maxima, histograms and sums through each other's shared memory; the first one
-// decides. Four CTAs of an SM, mostly of different rows, cover each other's loads
-// and exchanges. Bound: reading the logits; in practice the exponential and the
-// two conversions of each token (16 a cycle and SM), and the exchanges' latency.
-//
-// sample_long_kernel: a row of more than 65536 logits by one CTA that reads it
-// several times (the same steps, the histogram refined by further passes). It is
-// also how a row of sample_kernel ends whose cut lies among more than 2048 tokens
-// of one bin (many equal logits).
+// sample_kernel: a CTA has a row and reads it from memory once, for the maximum,
+// and then once or a few times more from the L2 cache (or L1):
+//   top-k     Every thread keeps the maximum of its own tokens. The k-th largest
+//             of these is no more than the k-th largest token, and little less
+//             when k is small against the threads, so its bin bounds the tokens
+//             to gather: a histogram of one entry a thread. They are sorted, and
+//             top-p, min-p and the draw go by that list alone.
+//   top-p     (without top-k) A histogram of the weights; the tokens of the bin
+//             where the cut lies are gathered and sorted.
+//   the rest  Sums of the kept weights by warp, each with a segment of the row;
+//             the warp that has the drawn sum walks through its segment.
+// A list of more than 2048 tokens (many equal logits) is cut by refining the
+// histogram instead (long_row). Bound: reading the logits; in practice, for few
+// rows the latency of the passes, for many the exponential and the conversions of
+// each token (16 a cycle and SM).
 #include <cstdint>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "engine.cuh"
@@ -35,13 +40,10 @@ constexpr float kSteps = 1048576.f;       // key steps per unit of depth
 constexpr float kLive = 32.f * kSteps;    // keys from here on weigh nothing: 2^31 · 2^-32 rounds to 0
 constexpr float kOne = 2147483648.f;      // the weight of key 0
 constexpr int kBins = 1024;               // of the histogram: 2^15 keys each
-constexpr int kThreads = 256;             // sample_kernel
-constexpr int kWarps = kThreads / 32;
-constexpr int kPer = 32;                  // logits of a thread
-constexpr int kSlice = kThreads * kPer;
-constexpr int kMaxCtas = 8;
 constexpr int kList = 2048;               // gathered tokens
-constexpr int kLongThreads = 1024;        // sample_long_kernel
+constexpr int kTail = 256;                // threads that sort the gathered tokens and draw from them
+constexpr float kNear = 16.f * kSteps;    // the depth of a first histogram
+constexpr int kAhead = 4;                 // vectors of 16 bytes that a thread loads at a time
 
 struct SampleArgs {
   const void* logits;
@@ -60,6 +62,7 @@ struct SampleArgs {
 struct Params {
   float m, c;        // the maximum; log2(e) / T · kSteps
   bool cold;         // T <= 0: the first of the largest logits
+  bool flat;         // cold, or a maximum or c of inf: only the largest logits weigh anything
   int k;             // 0: off
   float p;           // 1: off
   uint32_t least;    // min-p as a weight
@@ -89,9 +92,8 @@ __device__ __forceinline__ float key_of(float x, float m, float c) {
   const float d = (m - x) * c;
   return d < 8388608.f ? __fadd_rn(__fadd_rn(d, 8388608.f), -8388608.f) : d;
 }
-// The same in rows that are cold, or whose maximum is inf: only the largest logits count.
 __device__ __forceinline__ float key_of(float x, const Params& q) {
-  if (q.cold || q.m == INFINITY) return x == q.m ? 0.f : INFINITY;
+  if (q.flat) return x == q.m ? 0.f : INFINITY;
   return key_of(x, q.m, q.c);
 }
 __device__ __forceinline__ uint32_t weight_of(float key) {
@@ -187,12 +189,25 @@ __device__ __forceinline__ void put_none(const SampleArgs& a, int r) {
   if (a.logprobs) a.logprobs[r] = __int_as_float(0x7fc00000);
 }
 
+__device__ __forceinline__ uint32_t bits_of(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t bits_of(__half x) { return __half_as_ushort(x); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+template <typename T>
+__device__ __forceinline__ float from_bits(uint32_t b) {
+  if constexpr (sizeof(T) == 4)
+    return __uint_as_float(b);
+  else if constexpr (std::is_same<T, __half>::value)
+    return __half2float(__ushort_as_half((unsigned short)b));
+  else
+    return __uint_as_float(b << 16);
+}
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 // ---------------------------------------------------------------------------
-// One CTA for a row in global memory.
+// The cut by a refined histogram, for rows with more tokens near it than the list
+// holds.
 // ---------------------------------------------------------------------------
 template <int NT>
 struct LongMem {
@@ -309,7 +324,7 @@ __device__ void walk(const SampleArgs& a, int r, const T* x, const Params& q, in
 }
 
 template <int NT, typename T>
-__device__ __noinline__ void long_row(LongMem<NT>& s, const SampleArgs& a, int r, const T* x, const Params& q) {
+__device__ __noinline__ void long_row(LongMem<NT>& s, SampleArgs a, int r, const T* x, Params q) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Cut cut = kNoCut;
   if (q.cold || q.k || q.p < 1.f) {
@@ -346,445 +361,528 @@ __device__ __noinline__ void long_row(LongMem<NT>& s, const SampleArgs& a, int r
   if (run <= aim && aim < run + w) walk(a, r, x, q, lo, hi, cut, run, aim, total);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLongThreads) sample_long_kernel(SampleArgs a) {
-  __shared__ LongMem<kLongThreads> s;
-  __shared__ float s_m[kLongThreads / 32];
-  pdl_enter();
-  const int r = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + (long long)r * a.ld;
-  float m = -INFINITY;
-  for (int j = threadIdx.x; j < a.vocab; j += kLongThreads) m = fmaxf(m, to_float(x[j]));
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
-  __syncthreads();
-  for (int i = 0; i < kLongThreads / 32; ++i) m = fmaxf(m, s_m[i]);
-  if (m == -INFINITY) {
-    if (threadIdx.x == 0) put_none(a, r);
-    return;
-  }
-  Params q = params_of(a, r);
-  q.m = m;
-  long_row<kLongThreads, T>(s, a, r, x, q);
-}
-
 // ---------------------------------------------------------------------------
-// A cluster for a row, its logits in registers.
+// sample_kernel.
 // ---------------------------------------------------------------------------
-struct Histograms {
-  // this CTA's histogram; a bin's weight in 16-bit halves (of at most 8192 tokens, so neither sum passes 32 bits)
-  uint32_t count[kBins], high[kBins], low[kBins];
-  // first CTA: the row's
-  uint32_t all_count[kBins];
-  u64 all_weight[kBins];
-};
-struct Ranks {  // first CTA, when the histograms have been used: of the gathered tokens
-  u64 w_before[kList];
-  uint32_t rank[kList];
-};
+template <int NT>
 struct Mem {
   union {
-    Histograms h;
-    Ranks g;
+    struct {
+      uint32_t count[kBins];
+      uint32_t piece[3][kBins];  // weights, in pieces of so few bits that no sum passes 32
+    } h;
+    struct {
+      u64 list[kList];
+      int32_t queue[kList];  // vectors that may hold tokens of the list
+    };
+    LongMem<NT> far;
   };
-  // first CTA: the gathered tokens and their weights
-  u64 list[kList];
-  uint32_t list_w[kList];
-  uint32_t listed;
-  Scan<kThreads> scan;
-  // exchanged: by rank
-  float m[kMaxCtas];
-  u64 w[kMaxCtas];
-  // decided by the first CTA
-  int lo_bin, hi_bin, k_bin;  // gather the tokens of bins lo..hi, and of k_bin
+  uint32_t listed, queued;
+  u64 warp[NT / 32], total;
+  float warp_m[NT / 32];
+  int bin;
+  u64 before;
   Cut cut;
-  int long_way;
-  // of the warps
-  float warp_m[kWarps];
-  u64 warp_w[kWarps], warp_c[kWarps];
 };
 
-template <typename V>
-__device__ __forceinline__ V* remote(V* p, uint32_t rank) {  // the same variable of another CTA of the cluster
-  uint64_t g;
-  asm("mapa.u64 %0, %1, %2;" : "=l"(g) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
-  return reinterpret_cast<V*>(g);
+// A barrier of the first N threads: all NT, or the tail.
+template <int NT, int N>
+__device__ __forceinline__ void sync_n() {
+  asm volatile("bar.sync %0, %1;" ::"n"(N == NT ? 0 : 1), "n"(N) : "memory");
 }
 
-// Over the CTA: the sum of x and the maximum of y.
-__device__ __forceinline__ void block_sum_max(Mem& s, u64& x, u64& y) {
-  x = warp_sum(x);
-  for (int o = 16; o; o >>= 1) {
-    const u64 z = __shfl_xor_sync(~0u, y, o);
-    y = z > y ? z : y;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) {
-    s.warp_w[threadIdx.x >> 5] = x;
-    s.warp_c[threadIdx.x >> 5] = y;
-  }
-  __syncthreads();
-  x = y = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    x += s.warp_w[i];
-    y = s.warp_c[i] > y ? s.warp_c[i] : y;
-  }
-}
-
-// The row's cut, from the gathered tokens (whole bins) and the sums before top-k's and top-p's bins: the first CTA, all
-// its threads. Every token's rank and the weight before it come by comparing it with every other one.
-__device__ __forceinline__ Cut list_cut(Mem& s, int k, float p, const Found& fk, const Found& fp, u64 all_w) {
-  const uint32_t n = s.listed;
-  u64 earlier_bins = 0;  // gathered tokens of bins before top-k's
-  __syncthreads();       // (every thread has its histogram figures)
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-    const u64 me = s.list[i];
-    uint32_t rank = 0;
-    u64 before = 0;
-#pragma unroll 4
-    for (uint32_t j = 0; j < n; ++j) {
-      const bool ahead = s.list[j] < me;
-      rank += ahead;
-      before += ahead ? s.list_w[j] : 0u;
-    }
-    s.g.rank[i] = rank;
-    s.g.w_before[i] = before;
-    earlier_bins += (int)(me >> 36) < fk.bin;
-  }
-  Cut cut = kNoCut;
-  u64 kept = all_w, last = 0;
-  if (fk.bin < kBins) {
-    block_sum_max(s, earlier_bins, last);
-    kept = last = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-      const u64 me = s.list[i];
-      if ((int)(me >> 36) == fk.bin && fk.count + s.g.rank[i] - earlier_bins < (u64)k) {
-        kept += s.list_w[i];
-        last = me > last ? me : last;
-      }
-    }
-    block_sum_max(s, kept, last);
-    kept += fk.weight;
-    cut = last;
-  }
-  if (p < 1.f) {
-    const u64 aim = max(p_aim(p, kept), (u64)1);
-    last = kept = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-      const u64 me = s.list[i];
-      const int b = (int)(me >> 36);
-      if (b >= s.lo_bin && b <= s.hi_bin && fp.weight + s.g.w_before[i] < aim) last = me > last ? me : last;
-    }
-    block_sum_max(s, kept, last);
-    cut = last < cut ? last : cut;
-  }
-  return cut;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleArgs a, int ctas) {
-  constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec;
-  extern __shared__ __align__(16) uint8_t smem[];
-  Mem& s = *reinterpret_cast<Mem*>(smem);
-  // (no CTA writes to another one before that has started: the barrier's other half comes before the first write)
-  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  pdl_enter();
+// Sum of x over the threads before this one, and over all N.
+template <int NT, int N>
+__device__ __forceinline__ u64 block_scan(Mem<NT>& s, u64 x, u64& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = ctas > 1 ? cluster_ctarank() : 0;
-  const int r = blockIdx.x / ctas;
-  const T* row = static_cast<const T*>(a.logits) + (long long)r * a.ld;
-  Params q = params_of(a, r);
-  // A CTA's slice goes by 16-byte vectors, so the row begins `skew` places into the first one. Index order is that of
-  // (rank, warp, load, lane, place in the vector).
-  const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-  const int first = (int)rank * kSlice + warp * (32 * kPer) + lane * kVec - skew;
-  float x[kPer];
+  auto scan = [&](u64 v) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int j = first + i * 32 * kVec;
-    if (j >= 0 && j + kVec <= a.vocab) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + j));
-      const T* e = reinterpret_cast<const T*>(&v);
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 p = __shfl_up_sync(~0u, v, o);
+      if (lane >= o) v += p;
+    }
+    return v;
+  };
+  const u64 inc = scan(x);
+  sync_n<NT, N>();
+  if (lane == 31) s.warp[warp] = inc;
+  sync_n<NT, N>();
+  if (warp == 0) {
+    const u64 own = lane < N / 32 ? s.warp[lane] : 0, upto = scan(own);
+    if (lane < N / 32) s.warp[lane] = upto - own;
+    if (lane == 31) s.total = upto;
+  }
+  sync_n<NT, N>();
+  total = s.total;
+  return s.warp[warp] + inc - x;
+}
+
+// The first bin at which the running sum of of(bin) reaches aim (> 0), kBins if none; s.before: the sum before it.
+template <int NT, typename F, typename A>
+__device__ __forceinline__ int first_bin(Mem<NT>& s, u64& total, F&& of, A&& aim_of_total) {
+  constexpr int kEach = kBins / NT;
+  u64 v[kEach], sum = 0;
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) x[i * kVec + k] = to_float(e[k]);
+  for (int i = 0; i < kEach; ++i) sum += v[i] = of(threadIdx.x * kEach + i);
+  if (threadIdx.x == 0) s.bin = kBins;
+  u64 before = block_scan<NT, NT>(s, sum, total);
+  const u64 aim = aim_of_total(total);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (before < aim && before + v[i] >= aim) {  // one bin at most
+      s.bin = threadIdx.x * kEach + i;
+      s.before = before;
+    }
+    before += v[i];
+  }
+  __syncthreads();
+  return s.bin;
+}
+
+// Sorts list[0, n) upwards, by the tail's threads (bitonic); places up to the next power of two are overwritten. Strides
+// below 32 go by shuffles.
+template <int NT>
+__device__ __forceinline__ void sort_list(u64* list, int n) {
+  const int lane = threadIdx.x & 31;
+  int places = 32;
+  while (places < n) places *= 2;
+  for (int i = n + threadIdx.x; i < places; i += kTail) list[i] = ~0ull;
+  sync_n<NT, kTail>();
+#pragma unroll 1
+  for (int size = 32; size <= places; size *= 2) {
+#pragma unroll 1
+    for (int stride = size / 2; stride >= 32; stride /= 2) {
+      for (int t = threadIdx.x; t < places / 2; t += kTail) {
+        const int i = 2 * t - (t & (stride - 1));
+        const u64 x = list[i], y = list[i + stride];
+        if ((x > y) == !(i & size)) {
+          list[i] = y;
+          list[i + stride] = x;
+        }
+      }
+      sync_n<NT, kTail>();
+    }
+    for (int i = threadIdx.x; i - lane < places; i += kTail) {
+      u64 x = list[i];
+      auto strides = [&](int of, int first) {
+#pragma unroll
+        for (int stride = first; stride; stride /= 2) {
+          const u64 y = __shfl_xor_sync(~0u, x, stride);
+          const bool least = !(i & stride) == !(i & of);
+          x = least == (y < x) ? y : x;
+        }
+      };
+      if (size == 32) {  // the smaller sizes first
+        strides(2, 1);
+        strides(4, 2);
+        strides(8, 4);
+        strides(16, 8);
+      }
+      strides(size, 16);
+      list[i] = x;
+    }
+    sync_n<NT, kTail>();
+  }
+}
+
+// A row as vectors of 16 bytes: it begins `skew` places into the first one, if it does not begin on 16 bytes.
+template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* x;
+  int skew, vocab, lo, hi;  // the warp's segment, in vectors
+  __device__ __forceinline__ int index(int v) const { return v * kVec - skew; }
+  // the vector whose first token is j; places outside [0, end) are -inf
+  __device__ __forceinline__ uint4 load_at(int j, int end) const {
+    if (j >= 0 && j + kVec <= end) return *reinterpret_cast<const uint4*>(x + j);
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      w[k * sizeof(T) / 4] |= (j + k >= 0 && j + k < end ? bits_of(x[j + k]) : bits_of(T(-INFINITY)))
+                              << (k * sizeof(T) % 4 * 8);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // v and those 32, 64, ... further (for the warp's 32 lanes in a row)
+  __device__ __forceinline__ void load(int v, uint4 (&e)[kAhead]) const {
+    const int v0 = v - (int)(threadIdx.x & 31);
+    if (v0 >= (skew != 0) && v0 + 32 * kAhead <= min(hi, (vocab + skew) / kVec)) {
+      const uint4* p = reinterpret_cast<const uint4*>(x - skew) + v;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) e[i] = p[32 * i];
     } else {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) x[i * kVec + k] = j + k >= 0 && j + k < a.vocab ? to_float(row[j + k]) : -INFINITY;
+      for (int i = 0; i < kAhead; ++i) e[i] = load_at(index(v + 32 * i), v + 32 * i < hi ? vocab : 0);
     }
   }
-  if (threadIdx.x < 3) s.scan.found[threadIdx.x] = {kBins, 0, 0};
-  if (threadIdx.x == 0) s.listed = 0;
-  // the row's maximum
-  float m = x[0];
+  static __device__ __forceinline__ float value(const uint4& e, int k) {
+    const uint32_t w = k * sizeof(T) / 4 == 0 ? e.x : k * sizeof(T) / 4 == 1 ? e.y : k * sizeof(T) / 4 == 2 ? e.z : e.w;
+    return from_bits<T>(w >> (k * sizeof(T) % 4 * 8));
+  }
+  static __device__ __forceinline__ float most(const uint4& e) {  // the maximum of the vector
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(value(e, 0), value(e, 1)), fmaxf(value(e, 2), value(e, 3)));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      auto two = [](uint32_t w) { return *reinterpret_cast<T2*>(&w); };
+      const T2 m = __hmax2(__hmax2(two(e.x), two(e.y)), __hmax2(two(e.z), two(e.w)));
+      return fmaxf(to_float(m.x), to_float(m.y));
+    }
+  }
+  // f(index of the first, values), for the lane's vectors of the warp's segment, in order. (A long f's code is there
+  // once: four copies are slower by their way through the instruction cache, as most rows run them a few times only.)
+  template <bool kLong = true, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int v = lo + lane; v - lane < hi; v += 32 * kAhead) {
+      uint4 e[kAhead];
+      load(v, e);
+      if constexpr (kLong) {
+#pragma unroll 1
+        for (int i = 0; i < kAhead && v - lane + 32 * i < hi; ++i) {
+          f(index(v + 32 * i), e[0]);
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
+          for (int n = 1; n < kAhead; ++n) e[n - 1] = e[n];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f(index(v + 32 * i), e[i]);
+      }
+    }
+  }
+};
+
+// A logit that no token of a key up to `key` is below: the key's, less what rounding may have taken from it (2^-24 of
+// the difference, of the product and of m - x here, each).
+__device__ __forceinline__ float least_logit(float key, const Params& q) {
+  if (q.flat) return q.m;
+  const float d = (key + 1.f) / q.c;
+  return q.m - d - (fabsf(q.m) + d) * 0x1p-20f;
+}
+
+// Gathers the tokens of keys [from, to): the vectors that may hold some are queued, and then taken one a thread. False
+// if there are more than the list or the queue holds.
+template <int NT, typename T>
+__device__ __forceinline__ bool gather(Mem<NT>& s, const Row<T>& row, const Params& q, float from, float to) {
+  constexpr int kVec = Row<T>::kVec;
+  if (threadIdx.x == 0) s.listed = s.queued = 0;
+  __syncthreads();  // (the histogram is done with, too)
+  const float low = least_logit(to, q);
+  row.template each<false>([&](int j, const uint4& e) {
+    if (Row<T>::most(e) >= low) {
+      const uint32_t at = atomicAdd(&s.queued, 1u);
+      if (at < kList) s.queue[at] = j;
+    }
+  });
+  __syncthreads();
+  const int queued = (int)s.queued;
+  if (queued > kList) return false;
+#pragma unroll 1
+  for (int t = threadIdx.x; t < queued; t += NT) {
+    const int j = s.queue[t];
+    const uint4 e = row.load_at(j, row.vocab);
+    float key[kVec];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      key[k] = key_of(Row<T>::value(e, k), q);
+      mine |= (uint32_t)(key[k] >= from && key[k] < to) << k;
+    }
+    if (mine) {
+      uint32_t at = atomicAdd(&s.listed, (uint32_t)__popc(mine));
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        if (mine >> k & 1) {
+          if (at < kList) s.list[at] = token_of((uint32_t)key[k], j + k);
+          ++at;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  return s.listed <= kList;
+}
+
+// top-k's row, all of whose kept tokens are in the list, by the tail's threads.
+template <int NT>
+__device__ __forceinline__ void draw_from_list(Mem<NT>& s, const SampleArgs& a, int r, const Params& q, int k) {
+  constexpr int kEach = kList / kTail;
+  const int n = (int)s.listed, i0 = threadIdx.x * kEach;
+  sort_list<NT>(s.list, n);
+  u64 me[kEach], sum = 0, total;
+  uint32_t w[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const bool in = i0 + i < n && i0 + i < k;
+    me[i] = in ? s.list[i0 + i] : 0;
+    w[i] = in ? weight_of((float)(uint32_t)(me[i] >> 21)) : 0;
+    sum += w[i];
+  }
+  u64 before = block_scan<NT, kTail>(s, sum, total);
+  const u64 most = q.p < 1.f ? max(p_aim(q.p, total), (u64)1) : total;
+  u64 stay = 0;  // tokens: the first of the list
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const u64 next = before + w[i];
+    if (!(before < most && w[i] >= q.least)) w[i] = 0;
+    before = next;
+    stay += w[i] != 0;
+    sum += w[i];
+  }
+  block_scan<NT, kTail>(s, sum, total);
+  u64 kept;
+  block_scan<NT, kTail>(s, stay, kept);
+  // in index order
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (w[i]) s.list[i0 + i] = (me[i] & ((1u << 21) - 1)) << 32 | me[i] >> 21;
+  sync_n<NT, kTail>();
+  sort_list<NT>(s.list, (int)kept);
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    me[i] = i0 + i < (int)kept ? s.list[i0 + i] : 0;
+    w[i] = i0 + i < (int)kept ? weight_of((float)(uint32_t)me[i]) : 0;
+    sum += w[i];
+  }
+  u64 same;
+  before = block_scan<NT, kTail>(s, sum, same);
+  const u64 aim = aim_of(q.u, total);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (before <= aim && aim < before + w[i]) put(a, r, (int)(me[i] >> 32), (float)(uint32_t)me[i], total);
+    before += w[i];
+  }
+}
+
+// top-p's cut from the gathered tokens of its bin, by the tail's threads.
+template <int NT>
+__device__ __forceinline__ void cut_of_list(Mem<NT>& s, u64 before, u64 aim) {
+  constexpr int kEach = kList / kTail;
+  const int n = (int)s.listed, i0 = threadIdx.x * kEach;
+  sort_list<NT>(s.list, n);
+  uint32_t w[kEach];
+  u64 sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    w[i] = i0 + i < n ? weight_of((float)(uint32_t)(s.list[i0 + i] >> 21)) : 0;
+    sum += w[i];
+  }
+  before += block_scan<NT, kTail>(s, sum, total);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (before < aim && before + w[i] >= aim) s.cut = s.list[i0 + i];  // one token
+    before += w[i];
+  }
+}
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(SampleArgs a) {
+  constexpr int kVec = Row<T>::kVec, kWarps = NT / 32;
+  __shared__ __align__(16) Mem<NT> s;
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x;
+  Row<T> row;
+  row.x = static_cast<const T*>(a.logits) + (long long)r * a.ld;
+  row.vocab = a.vocab;
+  row.skew = (int)((reinterpret_cast<uintptr_t>(row.x) & 15u) / sizeof(T));
+  const int vectors = (a.vocab + row.skew + kVec - 1) / kVec, seg = (vectors + NT - 1) / NT * 32;
+  row.lo = min(vectors, warp * seg);
+  row.hi = min(vectors, row.lo + seg);
+  Params q = params_of(a, r);
+  // the thread's and the row's maximum
+  float mine = -INFINITY;
+  row.template each<false>([&](int, const uint4& e) {
+    mine = fmaxf(mine, Row<T>::most(e));
+  });
+  float m = mine;
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   if (lane == 0) s.warp_m[warp] = m;
+  for (int i = threadIdx.x; i < kBins; i += NT) s.h.count[i] = s.h.piece[0][i] = s.h.piece[1][i] = s.h.piece[2][i] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) m = fmaxf(m, s.warp_m[i]);
-  if (ctas > 1) {
-    asm volatile("barrier.cluster.wait;" ::: "memory");
-    if (threadIdx.x < ctas) *remote(&s.m[rank], threadIdx.x) = m;
-    cluster_sync();
-    for (int i = 0; i < ctas; ++i) m = fmaxf(m, s.m[i]);
-  }
-  if (m == -INFINITY || isnan(m)) {  // (every CTA of the row; a maximum over NaN alone is a NaN)
-    if (rank == 0 && threadIdx.x == 0) put_none(a, r);
+  if (m == -INFINITY) {  // (or NaN alone)
+    if (threadIdx.x == 0) put_none(a, r);
     return;
   }
   q.m = m;
-  if (q.cold || m == INFINITY) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = x[i] == m ? 0.f : INFINITY;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = key_of(x[i], q.m, q.c);
-  }
+  q.flat = q.cold || m == INFINITY || q.c == INFINITY;
 
-  Cut cut = kNoCut;
-  if (q.cold || q.k || q.p < 1.f) {
-    const bool by_p = !q.cold && q.p < 1.f;
-    const int k = q.cold ? 1 : q.k;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.h.count[i] = s.h.high[i] = s.h.low[i] = 0;
-    __syncthreads();
+  const int k = q.cold ? 1 : q.k;
+  u64 total;
+  if (k) {
+    // a bin that holds the k-th token, or a lower one: by the threads' maxima where k is small against them (half of
+    // them: 1.4 k tokens lie above it, if they are spread evenly), else by all tokens
+    auto count = [&](int b) -> u64 { return s.h.count[b]; };
+    auto all_of_k = [&](u64) -> u64 { return (u64)k; };
+    int bin = kBins;
+    if (2 * k <= NT) {
+      const float key = key_of(mine, q);
+      if (key < kLive) atomicAdd(&s.h.count[(uint32_t)key >> 15], 1u);
+      __syncthreads();
+      bin = first_bin<NT>(s, total, count, all_of_k);
+    }
+    float done = 0.f;  // the histogram begins at the tokens near the maximum, as long as these do
+    if (bin == kBins && 2 * k <= NT) {
+      for (int i = threadIdx.x; i < kBins; i += NT) s.h.count[i] = 0;
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (float depth = kNear; bin == kBins && done < kLive; depth = kLive) {
+      const float low = least_logit(depth, q);
+      row.each([&](int, const uint4& e) {
+        if (!(Row<T>::most(e) >= low)) return;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (x[i] < kLive) {
-        const uint32_t b = (uint32_t)x[i] >> 15;
-        atomicAdd(&s.h.count[b], 1u);
-        if (by_p) {
-          const uint32_t w = weight_of(x[i]);
-          atomicAdd(&s.h.high[b], w >> 16);
-          atomicAdd(&s.h.low[b], w & 0xffffu);
+        for (int i = 0; i < kVec; ++i) {
+          const float x = key_of(Row<T>::value(e, i), q);
+          if (x >= done && x < depth) atomicAdd(&s.h.count[(uint32_t)x >> 15], 1u);
         }
-      }
+      });
+      __syncthreads();
+      bin = first_bin<NT>(s, total, count, all_of_k);
+      done = depth;
     }
-    auto sync = [&]() {
-      if (ctas > 1)
-        cluster_sync();
-      else
-        __syncthreads();
+    if (bin < kBins) {  // (else fewer than k tokens weigh anything)
+      if (gather<NT, T>(s, row, q, 0.f, (float)((bin + 1) << 15))) {
+        if (threadIdx.x < kTail) draw_from_list<NT>(s, a, r, q, k);
+      } else {
+        long_row<NT, T>(s.far, a, r, row.x, q);
+      }
+      return;
+    }
+  }
+  Cut cut = kNoCut;
+  if (q.p < 1.f) {
+    // (of up to 2^16 tokens, 16 bits of each; of up to 2^21, 11)
+    const int bits = a.vocab <= 1 << 16 ? 16 : 11;
+    const uint32_t mask = (1u << bits) - 1;
+    auto weight = [&](int b) {
+      return s.h.piece[0][b] + ((u64)s.h.piece[1][b] << bits) + ((u64)s.h.piece[2][b] << 2 * bits);
     };
-    sync();
-    // the row's histogram: each CTA sums some bins over the cluster, into the first one's memory
-    const int each = (kBins + ctas - 1) / ctas;
-    for (int b = (int)rank * each + threadIdx.x; b < min(kBins, (int)(rank + 1) * each); b += kThreads) {
-      uint32_t c = 0;
-      u64 w = 0;
-#pragma unroll 4
-      for (int i = 0; i < ctas; ++i) {
-        c += *remote(&s.h.count[b], i);
-        if (by_p) w += ((u64) * remote(&s.h.high[b], i) << 16) + *remote(&s.h.low[b], i);
-      }
-      *remote(&s.h.all_count[b], 0) = c;
-      *remote(&s.h.all_weight[b], 0) = w;
-    }
-    sync();
-    // the first CTA: where the cuts lie. top-p's aim goes by what top-k keeps, known to within top-k's bin, so a few
-    // bins may hold it.
-    Found fk = {kBins, 0, 0}, fp = {kBins, 0, 0};
-    u64 all_w = 0;
-    if (rank == 0) {
-      u64 c, w;
-      scan_bins<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w);
-      if (k) {
-        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, true, (u64)k, 0);
-        __syncthreads();
-        fk = s.scan.found[0];
-      }
-      int lo = kBins, hi = -1;
-      if (by_p) {
-        for (int i = 0; i < kWarps; ++i) all_w += s.scan.w[i];
-        const u64 least_w = fk.bin < kBins ? fk.weight : all_w;
-        const u64 most_w = fk.bin < kBins ? fk.weight + s.h.all_weight[fk.bin] : all_w;
-        const u64 lo_aim = max(p_aim(q.p, least_w), (u64)1), hi_aim = max(p_aim(q.p, most_w), (u64)1);
-        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, lo_aim, 1);
-        find_bin<kThreads>(s.scan, s.h.all_count, s.h.all_weight, c, w, false, hi_aim, 2);
-        __syncthreads();
-        fp = s.scan.found[1];
-        lo = fp.bin;
-        hi = s.scan.found[2].bin;
-      }
-      if (threadIdx.x < ctas) {
-        *remote(&s.lo_bin, threadIdx.x) = lo;
-        *remote(&s.hi_bin, threadIdx.x) = hi;
-        *remote(&s.k_bin, threadIdx.x) = fk.bin;
-      }
-    }
-    sync();
-    if (s.k_bin < kBins || s.lo_bin < kBins) {
-      // (keys up to kLive only: a bin that is none begins there)
-      const float lo_key = (float)(s.lo_bin << 15), hi_key = (float)((s.hi_bin + 1) << 15);
-      const float k_lo = (float)(s.k_bin << 15), k_hi = s.k_bin < kBins ? (float)((s.k_bin + 1) << 15) : k_lo;
-      uint32_t* const listed = remote(&s.listed, 0);
-      u64* const list = remote(&s.list[0], 0);
-      uint32_t* const list_w = remote(&s.list_w[0], 0);
-      // (one atomic of each warp on the first CTA's count: a round trip takes about a thousand cycles)
-      uint32_t mine = 0;
+    // The histogram begins at the tokens near the maximum, the others' weights being summed alone; mostly these hold the
+    // cut, and the atomics for the many others are saved.
+    int bin = kBins;
+    u64 rest_of_all = 0;
+    auto aim_of_all = [&](u64 all) { return max(p_aim(q.p, all + rest_of_all), (u64)1); };
+    float done = 0.f;
+#pragma unroll 1
+    for (float depth = kNear; bin == kBins && done < kLive; depth = kLive) {
+      u64 rest = 0;
+      row.each([&](int, const uint4& e) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        mine |= (uint32_t)((x[i] >= lo_key && x[i] < hi_key) || (x[i] >= k_lo && x[i] < k_hi)) << i;
-      const uint32_t n = __popc(mine);
-      uint32_t at = n;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t p = __shfl_up_sync(~0u, at, o);
-        if (lane >= o) at += p;
-      }
-      uint32_t from = 0;
-      if (lane == 31 && at) from = atomicAdd(listed, at);
-      at += __shfl_sync(~0u, from, 31) - n;
-      if (__any_sync(~0u, n != 0)) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (mine >> i & 1) {
-            if (at < kList) {
-              list[at] = token_of((uint32_t)x[i], first + (i / kVec) * 32 * kVec + i % kVec);
-              list_w[at] = weight_of(x[i]);
-            }
-            at += 1;
+        for (int i = 0; i < kVec; ++i) {
+          const float x = key_of(Row<T>::value(e, i), q);
+          const uint32_t w = weight_of(x);
+          if (x >= done && x < depth) {
+            const uint32_t b = (uint32_t)x >> 15, low = w & mask, mid = w >> bits & mask;
+            if (low) atomicAdd(&s.h.piece[0][b], low);
+            if (mid) atomicAdd(&s.h.piece[1][b], mid);
+            if (bits < 16 && w >> 2 * bits) atomicAdd(&s.h.piece[2][b], w >> 2 * bits);
+          } else if (x >= depth) {
+            rest += w;
           }
         }
-      }
-      sync();
-      if (rank == 0) {
-        const bool too_many = s.listed > kList;
-        if (!too_many) cut = list_cut(s, k, by_p ? q.p : 1.f, fk, fp, all_w);
-        if (threadIdx.x < ctas) {
-          *remote(&s.cut, threadIdx.x) = cut;
-          *remote(&s.long_way, threadIdx.x) = too_many;
-        }
-      }
-      sync();
-      cut = s.cut;
-      if (s.long_way) {
-        if (rank == 0) long_row<kThreads, T>(*reinterpret_cast<LongMem<kThreads>*>(smem), a, r, row, q);
-        return;
-      }
+      });
+      block_scan<NT, NT>(s, rest, rest_of_all);
+      bin = first_bin<NT>(s, total, weight, aim_of_all);
+      done = depth;
     }
+    const u64 before = s.before;
+    if (!gather<NT, T>(s, row, q, (float)(bin << 15), (float)((bin + 1) << 15))) {
+      long_row<NT, T>(s.far, a, r, row.x, q);
+      return;
+    }
+    if (threadIdx.x < kTail) cut_of_list<NT>(s, before, aim_of_all(total));
+    __syncthreads();
+    cut = s.cut;
   }
 
-  // kept weight of every warp, CTA and the row
+  // kept weight of every warp and of the row
   const float cut_key = (float)(cut >> 21);
   const int cut_index = (int)(cut & ((1u << 21) - 1));
-  auto kept = [&](int i) -> uint32_t {  // weight of the thread's token i, 0 if it does not stay
-    const uint32_t y = stays(x[i], first + (i / kVec) * 32 * kVec + i % kVec, cut_key, cut_index) ? weight_of(x[i]) : 0;
+  auto kept = [&](float x, int j, float& key) -> uint32_t {  // weight of token j, 0 if it does not stay
+    key = key_of(x, q);
+    const uint32_t y = stays(key, j, cut_key, cut_index) ? weight_of(key) : 0;
     return y >= q.least ? y : 0;
   };
-  u64 w = 0;
-  if (cut == kNoCut && q.least == 0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) w += weight_of(x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; i += kVec) {  // (most loads of a row that is cut hold no token that stays)
-      float least_key = x[i];
-#pragma unroll
-      for (int k = 1; k < kVec; ++k) least_key = fminf(least_key, x[i + k]);
-      if (__any_sync(~0u, least_key <= cut_key)) {
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) w += kept(i + k);
-      }
-    }
-  }
-  w = warp_sum(w);
-  __syncthreads();
-  if (lane == 0) s.warp_w[warp] = w;
-  __syncthreads();
-  u64 total = 0, run = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i == warp) run = total;
-    total += s.warp_w[i];
-  }
-  if (ctas > 1) {
-    if (threadIdx.x < ctas) *remote(&s.w[rank], threadIdx.x) = total;
-    cluster_sync();
-    total = 0;
-    for (int i = 0; i < ctas; ++i) {
-      if (i == (int)rank) run += total;
-      total += s.w[i];
-    }
-  }
-  const u64 aim = aim_of(q.u, total);
-  if (aim < run || aim >= run + w) return;
-  // the warp that has it: the load, then the lane, then the token at which the running sum passes the aim
-  uint32_t y[kVec];
-  float key[kVec];
-  int j = 0;
-  bool here = false;
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    u64 sum = 0;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) sum += kept(i * kVec + k);
-    sum = warp_sum(sum);
-    if (!here) {
-      if (run + sum > aim) {
-        here = true;
-        j = first + i * 32 * kVec;
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          y[k] = kept(i * kVec + k);
-          key[k] = x[i * kVec + k];
-        }
-      } else {
-        run += sum;
-      }
-    }
-  }
+  const float low = least_logit(cut_key, q);
   u64 sum = 0;
+  float key;
+  if (cut == kNoCut && q.least == 0 && !q.flat)
+    row.template each<false>([&](int, const uint4& e) {
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) sum += y[k];
-  u64 inc = sum;
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 p = __shfl_up_sync(~0u, inc, o);
-    if (lane >= o) inc += p;
-  }
-  const uint32_t over = __ballot_sync(~0u, run + inc > aim);
-  if (lane != __ffs(over) - 1) return;
-  run += inc - sum;
+      for (int i = 0; i < kVec; ++i) sum += weight_of(key_of(Row<T>::value(e, i), q.m, q.c));
+    });
+  else
+    row.each([&](int j, const uint4& e) {
+      if (!(Row<T>::most(e) >= low)) return;
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    run += y[k];
-    if (run > aim) {
-      put(a, r, j + k, key[k], total);
-      return;
+      for (int i = 0; i < kVec; ++i) sum += kept(Row<T>::value(e, i), j + i, key);
+    });
+  u64 run = block_scan<NT, NT>(s, sum, total);
+  run = __shfl_sync(~0u, run, 0);
+  const u64 aim = aim_of(q.u, total);
+  sum = warp_sum(sum);
+  if (aim < run || aim - run >= sum) return;
+  // the warp that has it: the loads, then the load, the lane and the token at which the running sum passes the aim
+#pragma unroll 1
+  for (int v = row.lo + lane; v - lane < row.hi; v += 32 * kAhead) {
+    uint4 e[kAhead];
+    u64 own[kAhead], all = 0;
+    row.load(v, e);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      own[i] = 0;
+#pragma unroll
+      for (int n = 0; n < kVec; ++n) own[i] += kept(Row<T>::value(e[i], n), row.index(v + 32 * i) + n, key);
+      all += own[i];
+    }
+    all = warp_sum(all);
+    if (run + all <= aim) {
+      run += all;
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      u64 inc = own[i];
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 p = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += p;
+      }
+      const uint32_t over = __ballot_sync(~0u, run + inc > aim);
+      if (over) {
+        if (lane == __ffs(over) - 1) {
+          run += inc - own[i];
+#pragma unroll
+          for (int n = 0; n < kVec; ++n) {
+            const int j = row.index(v + 32 * i) + n;
+            const uint32_t y = kept(Row<T>::value(e[i], n), j, key);
+            if (run <= aim && aim < run + y) put(a, r, j, key, total);
+            run += y;
+          }
+        }
+        return;
+      }
+      run += __shfl_sync(~0u, inc, 31);
     }
   }
 }
 
 template <typename T>
 int launch_t(const SampleArgs& a, int rows, const DeviceCtx* c, cudaStream_t st) {
-  // (a row that does not begin on 16 bytes takes part of one more vector)
-  const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld * sizeof(T) % 16 == 0;
-  const int ctas = (a.vocab + (aligned ? 0 : (int)(16 / sizeof(T)) - 1) + kSlice - 1) / kSlice;
-  if (ctas > kMaxCtas) {
-    B2P_CHECK_CUDA(launch_pdl(sample_long_kernel<T>, dim3(rows), dim3(kLongThreads), 0, st, a));
-    B2P_POST_LAUNCH();
-    return B2P_OK;
-  }
-  static_assert(sizeof(LongMem<kThreads>) <= sizeof(Mem), "the long way fits the same memory");
-  static thread_local uint64_t attr_mask = 0;  // one per instantiation
-  if (!(attr_mask & (1ull << (c->device & 63)))) {
-    B2P_CHECK_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Mem)));
-    attr_mask |= 1ull << (c->device & 63);
-  }
-  B2P_REQUIRE((long long)rows * ctas < (1ll << 31), "too many rows in one call");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Mem);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  B2P_CHECK_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, ctas));
+  // As many threads for a row as leave all rows resident at once. Measured with 1024 / 512 / 256 threads: 64 rows of
+  // 49152 (top-k 200) 14 / 15 / 34 us, 148 of 32000 (unfiltered) 13 / 17 / 26; 256 of 49152 29 / 20 / 49, 296 of 32000
+  // 24 / 22 / 30; 1024 of 49152 (top-k 50) 85 / 50 / 40, 4096 of 2000 238 / 130 / 77.
+  const int sms = c->num_sms;
+  const int nt = rows <= sms ? 1024 : rows <= 2 * sms ? 512 : 256;
+  if (nt == 1024)
+    B2P_CHECK_CUDA(launch_pdl(sample_kernel<1024, T>, dim3(rows), dim3(1024), 0, st, a));
+  else if (nt == 512)
+    B2P_CHECK_CUDA(launch_pdl(sample_kernel<512, T>, dim3(rows), dim3(512), 0, st, a));
+  else
+    B2P_CHECK_CUDA(launch_pdl(sample_kernel<256, T>, dim3(rows), dim3(256), 0, st, a));
   B2P_POST_LAUNCH();
   return B2P_OK;
 }
