@@ -485,3 +485,36 @@ def test_sample_frequencies(b2p):
     tokens, _ = decode.sample(row.expand(n, vocab).contiguous(), u, temperature=torch.full((n,), 0.7, device="cuda"))
     seen = torch.bincount(tokens.long(), minlength=vocab) / n
     assert (seen - torch.softmax(row / 0.7, 0)).abs().max() <= 2.0 / n
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 5000), (160, 5000), (310, 5000), (2, 70001)])
+@pytest.mark.parametrize("std", [0.05, 3.0, 30.0])
+def test_sample_wide_filters(b2p, rows, vocab, std):
+    """top_k from a few to more than the threads, the list or the tokens that weigh anything; top_p to nearly 1."""
+    g = gen(rows + vocab)
+    logits = (randn(g, rows, vocab) * std).float()
+    u = torch.rand(rows, device="cuda", generator=g)
+    temp = torch.full((rows,), 0.7, device="cuda")
+    ks = torch.tensor([1, 100, 129, 300, 513, 1400, 2500, vocab - 1], device="cuda").int()
+    ps = torch.tensor([0.5, 0.9, 0.999, 0.9999999], device="cuda")
+    k = ks[torch.arange(rows, device="cuda") % 8].contiguous()
+    p = ps[torch.arange(rows, device="cuda") // 8 % 4].contiguous()
+    if rows == 2:
+        k, p = ks[[4, 6]].contiguous(), ps[[2, 3]].contiguous()
+    x = logits.cpu().numpy()
+    for kk, pp in ((k, None), (None, p), (k, p)):
+        tokens, logprobs = decode.sample(logits, u, temp, kk, pp)
+        for r in range(0, rows, max(1, rows // 32)):
+            check_draw(x[r], int(tokens[r]), float(logprobs[r]), float(u[r]), float(temp[r]),
+                       0 if kk is None else int(kk[r]), 1.0 if pp is None else float(pp[r]), 0.0)
+
+
+def test_sample_tiny_temperature(b2p):
+    """A temperature whose reciprocal is not finite leaves the largest logits alone."""
+    logits = torch.zeros(4, 1000, device="cuda")
+    logits[:, 100], logits[:, 900] = 1.0, 1.0
+    u = torch.tensor([0.0, 0.49, 0.51, 0.99], device="cuda")
+    for t in (1e-30, 1e-36, 1e-40):
+        tokens, logprobs = decode.sample(logits, u, torch.full((4,), t, device="cuda"))
+        assert tokens.tolist() == [100, 100, 900, 900]
+        assert torch.allclose(logprobs, torch.full_like(u, -math.log(2.0)))
