@@ -35,11 +35,17 @@ constexpr int kStep = 32;            // keys of one warp step
 constexpr int kPitch = kKvHeadDim + 4;  // floats of a row of O in shared memory
 constexpr int kMaxChunk = 4096;      // keys of one part
 constexpr int kMaxChunkPages = kMaxChunk / 8 + 1;
-constexpr int kTeamOneKeys = 2048;   // suffixes up to this go to single warps, in units of 128 or 256 keys
 constexpr float kSlack = 8.f;        // weights go up to 2^8 before a row's reference moves
 constexpr int kMinPart = 128;        // no part shorter: its join would cost what it saves
+constexpr int kSinglePages = 32;     // of a single warp's unit: a lane's each
 constexpr int kWant = kSms * 4;      // blocks wanted of each list
-constexpr int kTcRows = 64;          // rows from which the prefix goes to the tcgen05 kernel
+// The prefix goes to the tcgen05 kernel from this length on, or from so many rows times keys (8-bit or 16-bit cache; the
+// first pay for widening). Measured, 5 KV heads, attn_rows_kernel / tcgen05: int8, 1024 keys, 96 rows 10.7 / 12.2 us,
+// 192 rows 14.2 / 13.3; 4096 keys, 24 rows 12.6 / 13.8, 48 rows 16.7 / 14.3; 8192 keys, 6 rows 16.9 / 14.5; 32768 keys,
+// 96 rows 40 / 28, 768 rows 175 / 74. 16-bit, 1024 keys, 24 rows 8.6 / 8.8, 48 rows 9.5 / 9.1; 4096 keys, 6 rows 10.9 / 10.9,
+// 24 rows 12.7 / 11.2.
+constexpr int kTcKeys = 8192;
+constexpr long long kTcWork8 = 128 * 1024, kTcWork16 = 48 * 1024;
 
 __device__ __forceinline__ float rcp_sfu(float x) {
   float y;
@@ -109,27 +115,26 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
 
 // W warps share a unit of work (some rows, some keys): 1 where sequences are many and short, so that no warp waits
 // for another, else the block's 4, whose parts are joined in shared memory first. 
-template <typename T, int KIND, int MT, int W, bool FUSE>
+template <typename T, int KIND, int MT, int W>
 __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
-    attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status) {
+    attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status, bool after_tc) {
   extern __shared__ __align__(16) uint8_t s_ring[];
   using Mem = StepMem<KIND>;
   __shared__ int s_pages[W == 1 ? 1 : kMaxChunkPages];
   __shared__ __align__(16) float s_o[W == 1 ? 1 : W][W == 1 ? 1 : MT * 16][kPitch];
   __shared__ float2 s_ml[W][MT * 16];
-  __shared__ int s_last[MT * 16];
-  // After the tcgen05 kernel of the same call (!FUSE) the inputs are complete already and no part is shared with it:
-  // this kernel then waits for it only at the end, so that the join, which waits for this one, has both.
-  if (FUSE)
-    pdl_enter();
-  else
+  // After the tcgen05 kernel of the same call the inputs are complete already and no part is shared with it: this kernel
+  // then waits for it only at the end, so that the join, which waits for this one, has both.
+  if (after_tc)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  else
+    pdl_enter();
   const int warp = W == 1 ? 0 : threadIdx.x >> 5;  // in the team
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y;
   int u = W == 1 ? blockIdx.x * kRowWarps + (threadIdx.x >> 5) : blockIdx.x;
   if (W == 1 && u >= units) {
-    if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (after_tc) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   // this unit's rows [row0, row_end), keys [first, end), page list and part
@@ -162,7 +167,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
   // the page list, the length and Q come together
   const int sh = a.c.page_shift;
   const int pages = ((end - 1) >> sh) - (first >> sh) + 1;
-  int my_page = 0;  // (W 1: 256 keys at most, so 32 pages)
+  int my_page = 0;  // (W 1: kSinglePages at most)
   if (W == 1) {
     if (lane < pages) my_page = list[(first >> sh) + lane];
   } else {
@@ -201,12 +206,8 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
   if (!shared) {
     base_len = len;
     end = min(end, len);
-    if (first >= end) {
-      // No key here: another part's unit writes the rows, or, where there is none, the first suffix unit does.
-      if (first == 0 && a.suffix_part == 0)
-        for (int r = row0 + (W == 1 ? lane >> 4 : threadIdx.x >> 4); r < row_end; r += 2 * W)
-          join_row<T>(a, kvh, r, 0, threadIdx.x & 15);
-      if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (first >= end) {  // no key here
+      if (after_tc) asm volatile("griddepcontrol.wait;" ::: "memory");
       return;
     }
   }
@@ -465,38 +466,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
       if (d == 0) a.part_ml[at0 + r] = make_float2(top, sum);
     }
   }
-  // and, with the last part of a row, all of them
-  if (FUSE) __threadfence();
-  if (!FUSE) {
-  } else if (W > 1) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += kRowThreads) {
-      const int r = row0 + i;
-      if (shared && a.max_suffix > 0) len = suffix_len(a, r / span, status);
-      s_last[i] = row_complete(a, kvh, r, len) ? len : -1;
-    }
-    __syncthreads();
-    __threadfence();
-    for (int i = threadIdx.x >> 4; i < count; i += kRowThreads / 16)
-      if (s_last[i] >= 0) join_row<T>(a, kvh, row0 + i, s_last[i], threadIdx.x & 15);
-  } else {
-    __syncwarp();
-    if (shared && a.max_suffix > 0 && lane < count) len = suffix_len(a, (row0 + lane) / span, status);
-    const bool last = lane < count && row_complete(a, kvh, row0 + lane, len);
-    unsigned rows = __ballot_sync(~0u, last);
-    if (rows) __threadfence();
-    while (rows) {  // two at a time
-      const int r0 = __ffs(rows) - 1;
-      rows &= rows - 1;
-      const int r1 = rows ? __ffs(rows) - 1 : -1;
-      rows &= rows - 1;
-      const int r = lane < 16 ? r0 : r1;
-      const int n = __shfl_sync(~0u, len, r < 0 ? 0 : r);
-      if (r >= 0) join_row<T>(a, kvh, row0 + r, n, lane & 15);
-      __syncwarp();
-    }
-  }
-  if (!FUSE) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (after_tc) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // A half warp per row: join the row's parts (zeros where there is none).
@@ -516,7 +486,6 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 struct Plan {
   bool tc;  // the prefix goes to the tcgen05 kernel
   int team;  // warps that share a unit of attn_rows_kernel
-  bool fuse; // whoever writes a row's last part joins the row; else attn_join_kernel does
   int mt, prefix_tiles, suffix_tiles, n_suffix, suffix_chunk;
   PrefixSplit split;
   int suffix_part, parts;
@@ -529,10 +498,15 @@ int chunk_for(int len, int tiles, int want) {
   int chunk = ceil_div(ceil_div(len, n), kMinPart) * kMinPart;
   return chunk > kMaxChunk ? kMaxChunk : chunk;
 }
-Plan make_plan(int batch, int q_len, int group, int kv_heads, int prefix_len, int max_suffix) {
+int single_chunk(int len) {  // keys of a single warp's unit: about eight units, of 128 to 1024 keys
+  int chunk = kMinPart;
+  while (chunk < 1024 && chunk * 8 < len) chunk *= 2;
+  return chunk;
+}
+Plan make_plan(int batch, int q_len, int group, int prefix_len, int max_suffix, const KvView& c) {
   Plan p = {};
-  const int rows = batch * q_len * group;
-  p.tc = prefix_len > 0 && rows >= kTcRows;
+  const int rows = batch * q_len * group, kv_heads = c.kv_heads;
+  p.tc = prefix_len >= kTcKeys || (long long)rows * prefix_len >= (c.kind == B2P_KV_16 ? kTcWork16 : kTcWork8);
   p.mt = (p.tc || prefix_len == 0 ? q_len * group : rows) > 16 ? 2 : 1;
   p.prefix_tiles = ceil_div(rows, 16 * p.mt);
   p.suffix_tiles = ceil_div(q_len * group, 16 * p.mt);
@@ -547,19 +521,28 @@ Plan make_plan(int batch, int q_len, int group, int kv_heads, int prefix_len, in
   if (max_suffix > 0) {
     const long long teams = (long long)batch * p.suffix_tiles * kv_heads;
     p.suffix_chunk = chunk_for(max_suffix, (int)(teams < kWant ? teams : kWant), kWant);
-    if ((p.tc || prefix_len == 0) && teams >= kWant && max_suffix <= kTeamOneKeys) {
+    // Units of single warps where there are sequences enough to fill the GPU with them. Measured, 5 KV heads, teams of 4 /
+    // single warps: suffixes of 1000 alone, 8 sequences 9.6 / 9.1 us, 16 12.6 / 10.7, 64 22.7 / 16.1; of 8000, 16
+    // sequences 33 / 47, 32 55 / 51, 64 94 / 81; 32 sequences of 500 after 500 shared keys 14.5 / 12.8, 16 of 300 after
+    // 1000 10.7 / 11.4. Units of 128, 256, 512 keys for 256 suffixes of 512: 40 / 39 / 43, for 128 of 4096 101 / 88 / 84.
+    const int chunk = single_chunk(max_suffix), shared_chunk = single_chunk(p.tc ? 0 : prefix_len);
+    const bool many = teams >= kSms || ((p.tc || prefix_len == 0) && 2 * teams >= kSms && max_suffix <= 2048);
+    if (many && max(chunk, shared_chunk) <= kSinglePages << c.page_shift) {
       p.team = 1;
-      p.suffix_chunk = max_suffix <= kTeamOneKeys / 2 ? 128 : 256;
+      p.suffix_chunk = chunk;
+      if (!p.tc && prefix_len > 0) {
+        p.split.prefix_chunk = shared_chunk;
+        p.split.n_prefix = ceil_div(prefix_len, shared_chunk);
+      }
     }
     p.n_suffix = ceil_div(max_suffix, p.suffix_chunk);
   }
   p.suffix_part = p.split.n_prefix > p.split.n_last ? p.split.n_prefix : p.split.n_last;
   p.parts = p.suffix_part + p.n_suffix;
-  p.fuse = !p.tc && p.parts > 0;
   return p;
 }
 
-template <typename T, int KIND, int MT, int W, bool FUSE>
+template <typename T, int KIND, int MT, int W>
 int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   const long long prefix_units = p.tc ? 0 : (long long)p.split.n_prefix * p.prefix_tiles;
   const long long units = prefix_units + (long long)a.batch * p.n_suffix * p.suffix_tiles;
@@ -567,23 +550,22 @@ int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStre
   static thread_local uint64_t attr_mask = 0;  // one per instantiation
   constexpr int kSmem = StepMem<KIND>::kBlock;
   if (!(attr_mask & (1ull << (c->device & 63)))) {
-    B2P_CHECK_CUDA(cudaFuncSetAttribute(attn_rows_kernel<T, KIND, MT, W, FUSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    B2P_CHECK_CUDA(cudaFuncSetAttribute(attn_rows_kernel<T, KIND, MT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         kSmem));
     attr_mask |= 1ull << (c->device & 63);
   }
   const int blocks = W == 1 ? ceil_div((int)units, kRowWarps) : (int)units;
-  B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT, W, FUSE>, dim3(blocks, a.c.kv_heads), dim3(kRowThreads), kSmem,
-                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, (int)units, c->status));
+  B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT, W>, dim3(blocks, a.c.kv_heads), dim3(kRowThreads), kSmem,
+                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, (int)units, c->status, p.tc));
   B2P_POST_LAUNCH();
   return B2P_OK;
 }
 
-template <typename T, int KIND, bool FUSE>
+template <typename T, int KIND>
 int launch_w(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   if (p.team == 1)
-    return p.mt == 2 ? launch_rows<T, KIND, 2, 1, FUSE>(a, p, c, st) : launch_rows<T, KIND, 1, 1, FUSE>(a, p, c, st);
-  return p.mt == 2 ? launch_rows<T, KIND, 2, kRowWarps, FUSE>(a, p, c, st)
-                   : launch_rows<T, KIND, 1, kRowWarps, FUSE>(a, p, c, st);
+    return p.mt == 2 ? launch_rows<T, KIND, 2, 1>(a, p, c, st) : launch_rows<T, KIND, 1, 1>(a, p, c, st);
+  return p.mt == 2 ? launch_rows<T, KIND, 2, kRowWarps>(a, p, c, st) : launch_rows<T, KIND, 1, kRowWarps>(a, p, c, st);
 }
 
 template <typename T, int KIND>
@@ -592,8 +574,8 @@ int run_t(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t s
   if (p.tc) rc = launch_prefix_tc(a, std::is_same<T, __nv_bfloat16>::value, st);
   if (rc) return rc;
   if (p.n_suffix > 0 || (p.split.n_prefix > 0 && !p.tc))
-    rc = p.fuse ? launch_w<T, KIND, true>(a, p, c, st) : launch_w<T, KIND, false>(a, p, c, st);
-  if (rc || p.fuse) return rc;
+    rc = launch_w<T, KIND>(a, p, c, st);
+  if (rc) return rc;
   B2P_CHECK_CUDA(launch_pdl(attn_join_kernel<T>, dim3(ceil_div(a.rows, 8), a.c.kv_heads), dim3(128), 0, st, a,
                             c->status));
   B2P_POST_LAUNCH();
@@ -629,16 +611,16 @@ size_t b2p_attention_prefix_workspace(int batch, int q_len, int heads, int kv_he
   if (!sizes_ok(batch, q_len, heads, kv_heads, prefix_len, max_suffix)) return 0;
   // A bound that grows with every argument, so that the workspace of the largest call serves all: parts are
   // kTcStageKeys keys or longer, and there are about kWant blocks of 32 rows, or kSms of 256, or one per kMaxChunk keys,
-  // or at most 8 single-warp units a row.
+  // or single-warp units: at most 8 a row, or of 1024 keys.
   const long long rows = (long long)batch * q_len * heads;
   long long slots = 0;
   for (int len : {prefix_len, max_suffix}) {
     if (len == 0) continue;
     const long long by_length = rows * ceil_div(len, kTcStageKeys);
-    const long long by_blocks = (long long)kSms * 256 + rows * (10 + len / kMaxChunk);
+    const long long by_blocks = (long long)kSms * 256 + rows * (10 + len / 1024);
     slots += by_length < by_blocks ? by_length : by_blocks;
   }
-  return (size_t)slots * (kKvHeadDim * sizeof(float) + sizeof(float2)) + (size_t)rows * sizeof(int) + 256;
+  return (size_t)slots * (kKvHeadDim * sizeof(float) + sizeof(float2)) + 256;
 }
 
 int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, void* out, int ld_out, float* lse,
@@ -668,12 +650,10 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   B2P_REQUIRE(workspace && workspace_bytes >= need, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   B2P_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
   const int group = heads / a.c.kv_heads;
-  const Plan p = make_plan(batch, q_len, group, a.c.kv_heads, prefix_len, max_suffix);
+  const Plan p = make_plan(batch, q_len, group, prefix_len, max_suffix, a.c);
   const size_t all_rows = (size_t)batch * q_len * heads;
   const size_t uses = (size_t)p.parts * all_rows * (kKvHeadDim * sizeof(float) + sizeof(float2));
-  // the counts are at the end, where no call that shares the workspace keeps parts
-  const size_t counts = ((workspace_bytes & ~(size_t)15) - all_rows * sizeof(int)) & ~(size_t)15;
-  B2P_REQUIRE(uses <= counts, "workspace bound of %zu bytes does not hold %zu", need, uses);
+  B2P_REQUIRE(uses <= workspace_bytes, "workspace bound of %zu bytes does not hold %zu", need, uses);
   DeviceCtx* c = nullptr;
   if ((rc = ctx_get(&c))) return rc;
   a.q = q;
@@ -686,7 +666,6 @@ int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, voi
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o +
                                         (size_t)p.parts * a.rows * a.c.kv_heads * kKvHeadDim);
-  a.arrived = reinterpret_cast<int*>(static_cast<char*>(workspace) + counts);
   a.ld_q = ld_q;
   a.ld_out = ld_out;
   a.batch = batch;

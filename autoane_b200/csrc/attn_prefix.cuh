@@ -8,8 +8,8 @@ namespace b2p {
 // Rows of one KV head: r = (b * q_len + i) * group + g, for query i of sequence b and query head
 // kvh * group + g. A part is what one kernel block computes for some rows over some keys: the rows'
 // maximum score (log2 domain), sum of exponentials and unnormalised output. The first parts split the
-// prefix, those from max(n_prefix, n_last) on each sequence's suffix, every split a fixed number of keys. For
-// few rows whoever writes the last part of a row joins them all; else attn_join_kernel does.
+// prefix, those from max(n_prefix, n_last) on each sequence's suffix, every split a fixed number of keys.
+// attn_join_kernel joins a row's parts.
 struct PrefixSplit {
   int pair_rows;               // rows below it: n_prefix parts of prefix_chunk keys
   int n_prefix, prefix_chunk;
@@ -26,7 +26,6 @@ struct PrefixArgs : PrefixSplit {
   const int32_t* suffix_lens;
   float* part_o;    // [part][kv_heads * rows][64]
   float2* part_ml;  // [part][kv_heads * rows] (maximum, sum)
-  int* arrived;     // [kv_heads * rows] parts written so far; zero between calls
   long long ld_q, ld_out;
   int batch, q_len, group, rows;  // rows = batch * q_len * group, of one KV head
   int prefix_len, suffix_pitch, max_suffix;
@@ -114,15 +113,6 @@ __device__ __forceinline__ void join_row(const PrefixArgs& a, int kvh, int r, in
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2<T>(acc.x * inv, acc.y * inv), pack_h2<T>(acc.z * inv, acc.w * inv));
   if (a.lse && sub == 0)
     a.lse[(long long)token * a.c.kv_heads * a.group + h] = top == -INFINITY ? -INFINITY : ref + log2f(sum);
-}
-
-// After a block has written a part of row r (threads of the block are past a fence and a barrier since): whether it
-// was the row's last. The one that finds so joins the row; the count is back at zero then.
-__device__ __forceinline__ bool row_complete(const PrefixArgs& a, int kvh, int r, int len) {
-  int* n = a.arrived + (long long)kvh * a.rows + r;
-  if (atomicAdd(n, 1) + 1 != parts_of(a, r, len)) return false;
-  *n = 0;
-  return true;
 }
 
 }  // namespace b2p

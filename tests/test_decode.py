@@ -127,6 +127,24 @@ def test_workspace_serves_every_smaller_call():
         assert rc != ARG, _lib.load().b2p_last_error()
 
 
+def test_workspace_serves_every_cache():
+    """Nor does it depend on the pages or the kind of the cache."""
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible: these addresses are not real")
+    rng = random.Random(8)
+    size = lambda a, b: int(math.exp(rng.uniform(math.log(a), math.log(b + 1))))  # noqa: E731
+    for _ in range(4000):
+        heads, kv = rng.choice([(15, 5), (9, 3), (8, 2), (12, 12), (16, 1), (64, 1)])
+        batch, q_len = size(1, 600), size(1, 8)
+        prefix, suffix = rng.choice([0, size(1, 200000)]), rng.choice([0, size(1, 200000)])
+        bound = _lib.load().b2p_attention_prefix_workspace(batch, q_len, heads, kv, prefix, suffix)
+        kind = rng.choice([dict(kind=_lib.KV_16, k_scale=None, v_scale=None), dict()])
+        rc = attend(cache=desc(kv_heads=kv, page_size=8 << rng.randrange(8), **kind), ld_q=heads * 64,
+                    ld_out=heads * 64, heads=heads, batch=batch, q_len=q_len, prefix_len=prefix, max_suffix=suffix,
+                    suffix_pitch=1 << 20, nbytes=bound)
+        assert rc != ARG, _lib.load().b2p_last_error()
+
+
 def test_descriptor_matches_header():
     text = (Path(__file__).resolve().parents[1] / "include" / "b2p.h").read_text()
     for name, value in (("B2P_KV_16", _lib.KV_16), ("B2P_KV_INT8", _lib.KV_INT8), ("B2P_KV_E4M3", _lib.KV_E4M3)):

@@ -518,3 +518,18 @@ def test_sample_tiny_temperature(b2p):
         tokens, logprobs = decode.sample(logits, u, torch.full((4,), t, device="cuda"))
         assert tokens.tolist() == [100, 100, 900, 900]
         assert torch.allclose(logprobs, torch.full_like(u, -math.log(2.0)))
+
+
+@pytest.mark.parametrize("batch,q_len,heads,kv,kind,dtype,page,prefix,suffix", [
+    (40, 1, 15, 5, I8, F16, 64, 800, 300),     # single warps for the prefix and the suffixes
+    (150, 1, 4, 1, E4, BF16, 16, 130, 40),
+    (64, 2, 12, 4, I8, F16, 32, 0, 2500),      # suffixes alone, of several hundred keys a unit
+    (160, 1, 2, 1, F16, F16, 8, 0, 2400),      # pages too small for such units
+    (160, 1, 2, 1, I8, F16, 8, 100, 1500),
+    (1, 1, 15, 5, F16, F16, 64, 8192, 30),     # the tcgen05 kernel for a few rows
+    (2, 1, 9, 3, I8, BF16, 128, 9001, 0),
+    (1, 3, 16, 1, E4, F16, 16, 8300, 700),
+])
+def test_prefix_attention_divisions(b2p, batch, q_len, heads, kv, kind, dtype, page, prefix, suffix):
+    """Each way that the work is divided."""
+    test_prefix_attention(b2p, batch, q_len, heads, kv, kind, dtype, page, prefix, suffix, 1.0)
