@@ -6,7 +6,10 @@
 // join to out = sum e^(m_p - M) o_p / sum e^(m_p - M) l_p, M = max m_p, and the
 // log-sum-exp M + log(sum e^(m_p - M) l_p). The shared prefix is one part list
 // for the rows of all sequences at once (its keys are read once for the batch);
-// each sequence's suffix is another.
+// each sequence's suffix is another. A long prefix goes to attn_prefix_tc.cu.
+// attn_join_kernel joins the parts. (Joining where a row's last part is written,
+// behind a fence and a counter, took longer: 8 sequences of one query, 15 heads,
+// 1024 shared keys 13.3 us in place of 8.6, 16 over 4096 34 in place of 17.)
 //
 // attn_rows_kernel: each warp holds 16 or 32 query rows of one KV head and runs
 // over 32 keys at a time with mma.sync. Its keys and values come as they are
@@ -21,6 +24,11 @@
 //   w_j = exp2(s_j log2e + log2 y_j - M), M near the largest of the sums so far,
 // so that o = sum w_j code_j, l = sum w_j / y_j and out = o / l: the one rounding
 // to 16 bit is that of w_j, as without scales, however small the values are.
+//
+// Bound: for few rows the latency of a unit's loads and of the join; for many the
+// instructions around 16 x 8 tiles that hold 3 rows of 16 (group 3). 256 suffixes
+// of up to 512 int8 keys, 5 KV heads: 22 us beside 10 us of reading; 8 sequences
+// over 1023 + 129 keys: 9 us with the join.
 #include <cstdint>
 #include <type_traits>
 #include "attn_prefix.cuh"
@@ -42,8 +50,8 @@ constexpr int kWant = kSms * 4;      // blocks wanted of each list
 // The prefix goes to the tcgen05 kernel from this length on, or from so many rows times keys (8-bit or 16-bit cache; the
 // first pay for widening). Measured, 5 KV heads, attn_rows_kernel / tcgen05: int8, 1024 keys, 96 rows 10.7 / 12.2 us,
 // 192 rows 14.2 / 13.3; 4096 keys, 24 rows 12.6 / 13.8, 48 rows 16.7 / 14.3; 8192 keys, 6 rows 16.9 / 14.5; 32768 keys,
-// 96 rows 40 / 28, 768 rows 175 / 74. 16-bit, 1024 keys, 24 rows 8.6 / 8.8, 48 rows 9.5 / 9.1; 4096 keys, 6 rows 10.9 / 10.9,
-// 24 rows 12.7 / 11.2.
+// 96 rows 40 / 28, 768 rows 175 / 74. 16-bit, 1024 keys, 24 rows 8.6 / 8.8, 48 rows 9.5 / 9.1; 4096 keys, 6 rows
+// 10.9 / 10.9, 24 rows 12.7 / 11.2.
 constexpr int kTcKeys = 8192;
 constexpr long long kTcWork8 = 128 * 1024, kTcWork16 = 48 * 1024;
 
@@ -114,10 +122,11 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
 }
 
 // W warps share a unit of work (some rows, some keys): 1 where sequences are many and short, so that no warp waits
-// for another, else the block's 4, whose parts are joined in shared memory first. 
+// for another, else the block's 4, whose parts are joined in shared memory first.
 template <typename T, int KIND, int MT, int W>
 __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
-    attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status, bool after_tc) {
+    attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status,
+                     bool after_tc) {
   extern __shared__ __align__(16) uint8_t s_ring[];
   using Mem = StepMem<KIND>;
   __shared__ int s_pages[W == 1 ? 1 : kMaxChunkPages];

@@ -1,7 +1,7 @@
 // attn_prefix_tc.cu — the prefix part of attention over a shared prefix on the
-// tcgen05 tensor cores, for batches whose rows (sequences x queries x query heads
-// of one KV head) fill 128-row tiles. attn_prefix.cu has the formulas, the parts
-// and the join.
+// tcgen05 tensor cores, in tiles of 128 rows (sequences x queries x query heads of
+// one KV head). attn_prefix.cu has the formulas, the parts, the join and the rule
+// by which a prefix comes here.
 //
 // A CTA takes one part of the prefix for two row tiles, or for the one left over
 // when their number is odd. Keys and values come in stages of 128, widened to 16
@@ -17,7 +17,10 @@
 // tensor work to each), and after them the issue of all the instructions around
 // them. Row r of a tile is lane 32 (r % 4) + r / 4: the rows of a tile that is not
 // full are spread over the SM's four sub-partitions, and with 64 rows or fewer the
-// upper 16 lanes of each quarter are left out.
+// upper 16 lanes of each quarter are left out. Measured: 768 rows of 5 KV heads over
+// 32768 int8 keys 70 us (28 us of exponentials; two warps share a scheduler's unit
+// and weigh at 68% of its rate), 80 rows of 6 over 4001 16-bit keys 12.5 us, 64 rows
+// of 12 over 8192 e4m3 keys 16 us.
 //
 // ref need not be the maximum: any number near it gives the same quotient. It is
 // the next integer above the first unit's scores, and moves only when a unit's sum

@@ -7,7 +7,8 @@
 // +- rot/16 and come by shuffles of the 16-bit pairs as loaded. A warp has
 // four tokens and goes through their heads together, so that it need not diverge
 // between Q, K and V and loads a token's angles once.
-// Bound: the reads and writes (65536 tokens of 15 / 5 heads to int8: 380 MB).
+// Bound: the reads and writes. 65536 tokens of 15 / 5 heads to int8: append 380 MB in
+// 69 us (5.5 TB/s), read back 131 MB in 23 us (5.6 TB/s).
 #include <cstdint>
 #include "decode.cuh"
 #include "ptx.cuh"
@@ -273,7 +274,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(ReadArgs a, uint32_
 template <typename T, int KIND, int MODE>
 int append_mode(const AppendArgs& a, const DeviceCtx* c, cudaStream_t st) {
   // One head a warp while that does not fill the GPU four times over: a warp that goes through 25 heads takes longer
-  // than the whole call of a few tokens.
+  // than the whole call of a few tokens. Measured, 25 heads, one a warp / all: 8 tokens 1.8 / 6.2 us, 2051 5.0 / 7.4,
+  // 4096 8.3 / 10.2, 8192 14.7 / 11.3, 16384 32 / 19.
   const int total = a.heads + 2 * a.c.kv_heads;
   const long long quads = ((long long)a.n_tokens + 3) / 4;
   const bool one = quads * total <= (long long)c->num_sms * 64 * 4;

@@ -207,7 +207,7 @@ class PrefixAttention:
             raise ValueError("batch, q_len, heads, kv_heads, max_prefix or max_suffix out of range")
         self.batch, self.q_len, self.heads, self.kv_heads = batch, q_len, heads, kv_heads
         self.max_prefix, self.max_suffix = max_prefix, max_suffix
-        self.workspace = torch.zeros(size, dtype=torch.uint8, device=device)
+        self.workspace = torch.empty(size, dtype=torch.uint8, device=device)
         self._ws, self._ws_bytes = self.workspace.data_ptr(), size
 
     def __call__(self, q: torch.Tensor, cache: KVCache, prefix_pages: torch.Tensor | None, prefix_len: int,

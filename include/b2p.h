@@ -133,8 +133,9 @@ int b2p_attention_backward(const void* qkv, int ld_qkv, const void* out, const v
  * nothing. head_dim is 64, as in every model here.
  *
  * Indices that live on the device (slots, positions, page ids, lengths) are
- * checked by the kernels: an entry out of range is skipped and recorded, and
- * b2p_device_status then returns B2P_ERR_DEVICE.
+ * checked by the kernels: nothing out of range is read or written, the entry is
+ * recorded, and b2p_device_status then returns B2P_ERR_DEVICE. A token with a bad
+ * slot is not written; what else goes by a bad entry is undefined.
  * ====================================================================== */
 #define B2P_KV_16 0   /* keys and values in the compute dtype, no scales */
 #define B2P_KV_INT8 1 /* int8 codes, one fp32 scale per token and KV head */
@@ -195,10 +196,8 @@ int b2p_kv_read(const b2p_kv_cache* cache, const int32_t* slots, int n_tokens, v
  * device; max_suffix bounds its entries and suffix_pitch >=
  * ceil(max_suffix/page_size). Query head h reads KV head h / (heads/kv_heads).
  * `workspace` holds at least b2p_attention_prefix_workspace() bytes (16-byte
- * aligned) for sizes that are at least this call's in each argument. It has to
- * be zeroed once, before its first use and after a call that ended in a device
- * error; calls that share one pass the same workspace_bytes and must be ordered
- * by their stream. Results repeat bit for bit. */
+ * aligned) for sizes that are at least this call's in each argument; calls that
+ * share one must be ordered by their stream. Results repeat bit for bit. */
 int b2p_attention_prefix(const b2p_kv_cache* cache, const void* q, int ld_q, void* out, int ld_out, float* lse,
                          int batch, int q_len, int heads, const int32_t* prefix_pages, int prefix_len,
                          const int32_t* suffix_pages, int suffix_pitch, const int32_t* suffix_lens, int max_suffix,
