@@ -80,3 +80,28 @@ def test_complete(b2p):
     with pytest.raises(ValueError, match="prompt"):
         c.prefill(torch.zeros(71, dtype=torch.int64))
     decode.check()
+
+
+def test_graph_replays(b2p):
+    """A captured decoding step gives what the plain one gives."""
+    syn, mc, c = setup(70, batch=2, kv=torch.int8)
+    c.prefill(torch.arange(70, device="cuda") * 37 % 3000)
+    tokens, u = torch.tensor([5, 2900], device="cuda"), torch.tensor([0.2, 0.7], device="cuda")
+    k = torch.full((2,), 40, dtype=torch.int32, device="cuda")
+    want = decode.sample(c.step(tokens), u, top_k=k)
+    c.new = 0  # the same token again
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        decode.sample(c.step(tokens), u, top_k=k)
+        c.new = 0
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = decode.sample(c.step(tokens), u, top_k=k)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    decode.check()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    del graph
