@@ -22,8 +22,8 @@
 //             the warp that has the drawn sum walks through its segment.
 // A list of more than 2048 tokens (many equal logits) is cut by refining the
 // histogram instead (long_row). Bound: reading the logits; in practice, for few
-// rows the latency of the passes, for many the instructions of each token (the
-// exponential and its conversion, 16 a cycle and SM, and about a dozen others).
+// rows the latency of the passes, for many that of the second one's reads from L2 at
+// 32 warps an SM (issue 35%, the exponential's unit 30% busy).
 // Measured: a row of 49152 (top-k 50) 10 us, 33 rows of 16893 (top-p 0.95) 25 us, 256
 // rows of 49152 in 16 bit (top-k 200, top-p, min-p) 18 us, 1024 rows of 32000 in 32 bit
 // (unfiltered) 60 us, 2.2 TB/s. (A row held in the registers of a cluster of CTAs, read
@@ -684,6 +684,7 @@ __device__ __forceinline__ void cut_of_list(Mem<NT>& s, u64 before, u64 aim) {
   }
 }
 
+// (64 registers, 1024 threads an SM: with 48 or 40 for 5 or 6 blocks of 256, 1024 rows of 32000 take 65 / 69 us, not 60.)
 template <int NT, typename T>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(SampleArgs a) {
   constexpr int kVec = Row<T>::kVec, kWarps = NT / 32;
