@@ -3,7 +3,8 @@ sequences share a long prefix, and sampling.
 
 A thin layer over b2p_kv_append, b2p_kv_read, b2p_attention_prefix and
 b2p_sample (include/b2p.h has their definitions) for torch tensors. All work
-goes to torch's current stream of the tensors' device; nothing synchronises.
+goes to torch's current stream of the current device, which has to be the
+tensors' own (the library launches there); nothing synchronises.
 Argument errors raise `B2PError` (from the library) or `ValueError` (shapes and
 types of the tensors). Indices on the device (slots, positions, page ids,
 lengths) are checked there: `check()` raises if any was out of range.
@@ -49,6 +50,16 @@ def _raise(name: str, rc: int):
 
 
 _stream = torch._C._cuda_getCurrentRawStream  # of a device index
+_current = torch.cuda.current_device
+
+
+def _on(device: int) -> int:
+    """The current stream of the tensors' device. The library launches on the current device and keeps its status word
+    there, so another one is refused: a kernel would start on the wrong GPU with this one's addresses."""
+    if device != _current():
+        raise ValueError(f"the tensors are on cuda:{device}, the current device is cuda:{_current()}: make theirs "
+                         f"current (torch.cuda.set_device or torch.cuda.device) for the call")
+    return _stream(device)
 
 
 def _rows(t: torch.Tensor, name: str, dtypes=_DTYPE) -> torch.Tensor:
@@ -71,7 +82,8 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def check(stream: int | None = None) -> None:
-    """Wait for `stream` (default: the current one) and raise if a kernel recorded a bad index or a failed wait."""
+    """Wait for `stream` (default: the current one) and raise if a kernel on the current device recorded a bad index or
+    a failed wait."""
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
     _lib.call("b2p_device_status", stream)
@@ -152,7 +164,7 @@ class KVCache:
         `table` (see rope_table; None: no rotation) at `positions` (int32 [n]). Returns rotated Q [n, 64·heads]
         (`out`, which may be a view of qkv)."""
         n, cols = _rows(qkv, "qkv").shape
-        q_cols, dev = heads * HEAD_DIM, self._dev
+        q_cols, dev, stream = heads * HEAD_DIM, self._dev, _on(self._dev)
         if cols < q_cols + 2 * HEAD_DIM * self.kv_heads or qkv.get_device() != dev:
             raise ValueError(f"qkv must have {q_cols + 2 * HEAD_DIM * self.kv_heads} columns, on {self.device}")
         if out is None:
@@ -172,7 +184,7 @@ class KVCache:
         rc = _fn("b2p_kv_append")(
             self._ref, qkv.data_ptr(), _ld(qkv), heads, out.data_ptr(), ld_out,
             _vec(slots, "slots", torch.int32, n, dev), _vec(positions, "positions", torch.int32, n, dev), angles,
-            max_pos, rot, 1 if interleaved else 0, n, self._dtype(qkv.dtype), _stream(dev))
+            max_pos, rot, 1 if interleaved else 0, n, self._dtype(qkv.dtype), stream)
         if rc:
             _raise("b2p_kv_append", rc)
         return out
@@ -181,7 +193,7 @@ class KVCache:
              v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The K and V of `slots` (int32 [n]; negative: zeros) as [n, 64·kv_heads] of `dtype`."""
         n, cols, dev = slots.numel(), HEAD_DIM * self.kv_heads, self._dev
-        code = self._dtype(dtype)
+        code, stream = self._dtype(dtype), _on(dev)
         for name, t in (("k_out", k_out), ("v_out", v_out)):
             if t is not None and (t.shape != (n, cols) or t.dtype is not dtype or t.get_device() != dev):
                 raise ValueError(f"{name} must be {dtype} [{n}, {cols}] on {self.device}")
@@ -189,7 +201,7 @@ class KVCache:
         v = torch.empty_like(k) if v_out is None else _rows(v_out, "v_out")
         rc = _fn("b2p_kv_read")(self._ref, _vec(slots, "slots", torch.int32, n, dev), n, k.data_ptr(),
                                 cols if k_out is None else _ld(k), v.data_ptr(), cols if v_out is None else _ld(v),
-                                code, _stream(dev))
+                                code, stream)
         if rc:
             _raise("b2p_kv_read", rc)
         return k, v
@@ -218,6 +230,7 @@ class PrefixAttention:
         n, cols, dev = self.batch * self.q_len, self.heads * HEAD_DIM, cache._dev
         if _rows(q, "q").shape != (n, cols) or q.get_device() != dev or cache.kv_heads != self.kv_heads:
             raise ValueError(f"q must be [{n}, {cols}] on {cache.device}, the cache have {self.kv_heads} KV heads")
+        stream = _on(dev)
         if not 0 <= prefix_len <= self.max_prefix:
             raise ValueError(f"prefix_len must be from 0 to {self.max_prefix}")
         prefix = pages = lens = None
@@ -243,7 +256,7 @@ class PrefixAttention:
         rc = _fn("b2p_attention_prefix")(
             cache._ref, q.data_ptr(), ld_q, out.data_ptr(), _ld(_rows(out, "out")),
             None if lse is None else lse.data_ptr(), self.batch, self.q_len, self.heads, prefix, prefix_len, pages,
-            pitch, lens, most, cache._dtype(q.dtype), self._ws, self._ws_bytes, _stream(dev))
+            pitch, lens, most, cache._dtype(q.dtype), self._ws, self._ws_bytes, stream)
         if rc:
             _raise("b2p_attention_prefix", rc)
         return (out, lse) if return_lse else out
@@ -257,6 +270,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
     (int32 [n]; `out`) and the natural logs of their probabilities among the kept tokens (fp32 [n])."""
     n, vocab = _rows(logits, "logits", _LOGITS).shape
     dev = logits.get_device()
+    stream = _on(dev)
     if u is None:
         raise ValueError("u is needed")
     logprobs = torch.empty_like(u)
@@ -267,7 +281,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
         logits.data_ptr(), _ld(logits), n, vocab, _LOGITS[logits.dtype], _vec(u, "u", f32, n, dev),
         _vec(temperature, "temperature", f32, n, dev), _vec(top_k, "top_k", i32, n, dev),
         _vec(top_p, "top_p", f32, n, dev), _vec(min_p, "min_p", f32, n, dev), _vec(out, "out", i32, n, dev),
-        logprobs.data_ptr(), _stream(dev))
+        logprobs.data_ptr(), stream)
     if rc:
         _raise("b2p_sample", rc)
     return out, logprobs

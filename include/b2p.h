@@ -129,8 +129,8 @@ int b2p_attention_backward(const void* qkv, int ld_qkv, const void* out, const v
  * Decoding: a paged key/value cache, attention of a batch that shares a long
  * prefix, and sampling. The reference generates text with a numpy forward and
  * top-k sampling (generate.py:161); these are the device operators of such
- * a loop. All take device pointers, are asynchronous on `stream` and allocate
- * nothing. head_dim is 64, as in every model here.
+ * a loop. All take pointers and a stream of the current device, are asynchronous
+ * on `stream` and allocate nothing. head_dim is 64, as in every model here.
  *
  * Indices that live on the device (slots, positions, page ids, lengths) are
  * checked by the kernels: nothing out of range is read or written, the entry is
