@@ -231,6 +231,8 @@ class PrefixAttention:
         if _rows(q, "q").shape != (n, cols) or q.get_device() != dev or cache.kv_heads != self.kv_heads:
             raise ValueError(f"q must be [{n}, {cols}] on {cache.device}, the cache have {self.kv_heads} KV heads")
         stream = _on(dev)
+        if self.workspace.get_device() != dev:
+            raise ValueError(f"the workspace is on {self.workspace.device}, the cache on {cache.device}")
         if not 0 <= prefix_len <= self.max_prefix:
             raise ValueError(f"prefix_len must be from 0 to {self.max_prefix}")
         prefix = pages = lens = None

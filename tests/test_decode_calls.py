@@ -63,3 +63,13 @@ def test_tensors_of_another_device_are_refused(calls, monkeypatch, what):
     with pytest.raises(ValueError, match="cuda:1"):
         call()
     assert len(calls) == 1
+
+
+def test_workspace_of_another_device_is_refused(calls, monkeypatch):
+    """A PrefixAttention made on one device does not work on a cache of another."""
+    monkeypatch.setattr(decode, "_current", lambda: 1)
+    att = decode.PrefixAttention(1, 1, 1, 1, 8, 0, device="cpu")
+    calls.clear()
+    with pytest.raises(ValueError, match="workspace"):
+        att(on_1(1, 64), cache_1(), vec(1), 8, None, None)
+    assert not calls
