@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(AppendArgs a, uin
                          e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16);
         if (at0 >= 0) {
           *reinterpret_cast<uint2*>(codes + at * 64 + l * 8) = o;
-          if (l == 0) (is_v ? a.c.v_scale : a.c.k_scale)[at] = top * (1.0f / kTop);
+          // (an infinite value's vector too has a NaN scale: its codes are 0 and, for int8, no NaN can be one)
+          if (l == 0)
+            (is_v ? a.c.v_scale : a.c.k_scale)[at] = top < INFINITY ? top * (1.0f / kTop) : __int_as_float(0x7fc00000);
         }
       }
     }

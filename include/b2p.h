@@ -170,7 +170,7 @@ typedef struct {
  * 8-bit kinds: with A the largest |x| of a (token, head) vector, taken in fp32
  * after rotation, codes are x * (c / max(A, 1e-30)) rounded to nearest even
  * (c = 127 for int8, 448 for e4m3) and the scale is max(A, 1e-30) / c. A vector
- * with a non-finite value reads back as NaN. */
+ * with a non-finite value has a NaN scale and reads back as NaN. */
 int b2p_kv_append(const b2p_kv_cache* cache, const void* qkv, int ld_qkv, int heads, void* q_out, int ld_q,
                   const int32_t* slots, const int32_t* positions, const float* rope, int max_pos, int rot,
                   int interleaved, int n_tokens, int dtype, void* stream);
