@@ -121,9 +121,20 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
   }
 }
 
+// Takes the non-finite values out of a pair (zero in their place); true if there was one.
+template <typename T>
+__device__ __forceinline__ bool take_nonfinite(uint32_t& x) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  const uint32_t bad = __vcmpeq2(x & kExp, kExp);
+  x &= ~bad;
+  return bad != 0;
+}
+
 // W warps share a unit of work (some rows, some keys): 1 where sequences are many and short, so that no warp waits
-// for another, else the block's 4, whose parts are joined in shared memory first.
-template <typename T, int KIND, int MT, int W>
+// for another, else the block's 4, whose parts are joined in shared memory first. MIXED: there are keys that some rows
+// of a tile see and others do not, and their values may be infinite or NaN (beside the test for it in every kernel, 64
+// sequences of one query took 31.3 us in place of 30.0).
+template <typename T, int KIND, int MT, int W, bool MIXED>
 __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
     attn_rows_kernel(PrefixArgs a, int prefix_tiles, int suffix_tiles, int prefix_units, int units, uint32_t* status,
                      bool after_tc) {
@@ -233,6 +244,8 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
         lim[m][e] = end;
       min_lim = min(min_lim, lim[m][e]);
     }
+  // From here on some of the suffix's keys are seen by its later queries alone.
+  const int first_hidden = shared ? 1 << 30 : len - (a.q_len - 1);
   const int used_pages = ((end - 1) >> sh) - (first >> sh) + 1;
   if (W == 1) {
     my_page = checked(my_page, lane < used_pages);
@@ -318,6 +331,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
     }
     // scores in the log2 domain, masked where a row's keys end; the value's scale joins in
     const bool whole = key0 + kStep <= min_lim;
+    const bool mixed = MIXED && key0 + kStep > first_hidden;  // (the same in all lanes)
     float vi[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -331,8 +345,9 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
         kc[1] = __uint_as_float(ks.y) * kScaleLog2;
         vl[0] = log2_sfu(v0);
         vl[1] = log2_sfu(v1);
-        vi[j][0] = rcp_sfu(v0);
-        vi[j][1] = rcp_sfu(v1);
+        // (a NaN scale has the weights NaN already; where a row does not see the key, its weight of 0 must stay one)
+        vi[j][0] = fmaxf(rcp_sfu(v0), 0.f);
+        vi[j][1] = fmaxf(rcp_sfu(v1), 0.f);
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -397,6 +412,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
         l[m][e] += sum;
       }
     // O += w·V: pairs (key 2t, key 2t + 1) of a tile, channel 8g + n
+    bool odd = false;
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
       uint32_t vb[2][8];
@@ -420,10 +436,49 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
           widen4<T, KIND>(__byte_perm(x.y, y.y, 0x7362), vb[j][6], vb[j][7]);
         }
       }
+      if (mixed) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) odd |= take_nonfinite<T>(vb[0][n]) | take_nonfinite<T>(vb[1][n]);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < 8; ++n) mma16816<T>(o[m][n], pa[m][jj], vb[0][n], vb[1][n]);
+    }
+    if (mixed && __any_sync(~0u, odd)) {
+      // A product with a weight of 0 would bring a value that is not finite to rows that do not see it. Those values
+      // were left out above; here the rows that see them get them. (A thread's columns of O: channels 16t + n and
+      // 16t + 8 + n.)
+#pragma unroll 1
+      for (int k = 0; k < kStep; ++k) {
+        uint32_t x[8];  // the channels' pairs
+        if constexpr (KIND == B2P_KV_16) {
+          const uint4 a0 = lds16(src + Mem::v_at(k, 2 * t)), a1 = lds16(src + Mem::v_at(k, 2 * t + 1));
+          x[0] = a0.x, x[1] = a0.y, x[2] = a0.z, x[3] = a0.w, x[4] = a1.x, x[5] = a1.y, x[6] = a1.z, x[7] = a1.w;
+        } else {
+          const uint4 c = lds16(src + Mem::v_at(k, t));
+          widen4<T, KIND>(c.x, x[0], x[1]);
+          widen4<T, KIND>(c.y, x[2], x[3]);
+          widen4<T, KIND>(c.z, x[4], x[5]);
+          widen4<T, KIND>(c.w, x[6], x[7]);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; n += 2)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t rest = x[4 * c + n / 2];
+            const float2 v = H2<T>::to_f2(*reinterpret_cast<typename H2<T>::V*>(&x[4 * c + n / 2]));
+            if (!take_nonfinite<T>(rest)) continue;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (key0 + k >= lim[m][e]) continue;
+                if (!(fabsf(v.x) < INFINITY)) o[m][n][2 * e + c] += v.x;
+                if (!(fabsf(v.y) < INFINITY)) o[m][n + 1][2 * e + c] += v.y;
+              }
+          }
+      }
     }
     __syncwarp();
     fetch(i + Mem::kRing);
@@ -551,30 +606,31 @@ Plan make_plan(int batch, int q_len, int group, int prefix_len, int max_suffix, 
   return p;
 }
 
-template <typename T, int KIND, int MT, int W>
+template <typename T, int KIND, int MT, int W, bool MIXED>
 int launch_rows(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   const long long prefix_units = p.tc ? 0 : (long long)p.split.n_prefix * p.prefix_tiles;
   const long long units = prefix_units + (long long)a.batch * p.n_suffix * p.suffix_tiles;
   B2P_REQUIRE(units < (1ll << 31), "too much work for one call");
   static thread_local uint64_t attr_mask = 0;  // one per instantiation
   constexpr int kSmem = StepMem<KIND>::kBlock;
+  const auto kernel = attn_rows_kernel<T, KIND, MT, W, MIXED>;
   if (!(attr_mask & (1ull << (c->device & 63)))) {
-    B2P_CHECK_CUDA(cudaFuncSetAttribute(attn_rows_kernel<T, KIND, MT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kSmem));
+    B2P_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     attr_mask |= 1ull << (c->device & 63);
   }
   const int blocks = W == 1 ? ceil_div((int)units, kRowWarps) : (int)units;
-  B2P_CHECK_CUDA(launch_pdl(attn_rows_kernel<T, KIND, MT, W>, dim3(blocks, a.c.kv_heads), dim3(kRowThreads), kSmem,
-                            st, a, p.prefix_tiles, p.suffix_tiles, (int)prefix_units, (int)units, c->status, p.tc));
+  B2P_CHECK_CUDA(launch_pdl(kernel, dim3(blocks, a.c.kv_heads), dim3(kRowThreads), kSmem, st, a, p.prefix_tiles,
+                            p.suffix_tiles, (int)prefix_units, (int)units, c->status, p.tc));
   B2P_POST_LAUNCH();
   return B2P_OK;
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, bool MIXED>
 int launch_w(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t st) {
   if (p.team == 1)
-    return p.mt == 2 ? launch_rows<T, KIND, 2, 1>(a, p, c, st) : launch_rows<T, KIND, 1, 1>(a, p, c, st);
-  return p.mt == 2 ? launch_rows<T, KIND, 2, kRowWarps>(a, p, c, st) : launch_rows<T, KIND, 1, kRowWarps>(a, p, c, st);
+    return p.mt == 2 ? launch_rows<T, KIND, 2, 1, MIXED>(a, p, c, st) : launch_rows<T, KIND, 1, 1, MIXED>(a, p, c, st);
+  return p.mt == 2 ? launch_rows<T, KIND, 2, kRowWarps, MIXED>(a, p, c, st)
+                   : launch_rows<T, KIND, 1, kRowWarps, MIXED>(a, p, c, st);
 }
 
 template <typename T, int KIND>
@@ -582,8 +638,11 @@ int run_t(const PrefixArgs& a, const Plan& p, const DeviceCtx* c, cudaStream_t s
   int rc = B2P_OK;
   if (p.tc) rc = launch_prefix_tc(a, std::is_same<T, __nv_bfloat16>::value, st);
   if (rc) return rc;
-  if (p.n_suffix > 0 || (p.split.n_prefix > 0 && !p.tc))
-    rc = launch_w<T, KIND>(a, p, c, st);
+  if (p.n_suffix > 0 || (p.split.n_prefix > 0 && !p.tc)) {
+    constexpr bool kFinite = KIND == B2P_KV_INT8;  // whatever the codes
+    rc = kFinite || p.n_suffix == 0 || a.q_len == 1 ? launch_w<T, KIND, false>(a, p, c, st)
+                                                    : launch_w<T, KIND, !kFinite>(a, p, c, st);
+  }
   if (rc) return rc;
   B2P_CHECK_CUDA(launch_pdl(attn_join_kernel<T>, dim3(ceil_div(a.rows, 8), a.c.kv_heads), dim3(128), 0, st, a,
                             c->status));

@@ -7,11 +7,15 @@ import pytest
 import torch
 
 from autoane_b200 import decode
-from tests.test_gpu_decode import BF16, E4, F16, I8, gen, randn
+from tests.test_gpu_decode import BF16, E4, F16, I8, attend64, gen, make_cache, randn
 
 pytestmark = pytest.mark.gpu
 
 NAN, INF = math.nan, math.inf
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
 # ---- cache ----------------------------------------------------------------------------------------------------
@@ -50,4 +54,72 @@ def test_infinite_key_is_not_lost(b2p, kind, prefix, sign):
     att = decode.PrefixAttention(1, 1, 1, 1, prefix, 0)
     out, lse = att(q, cache, torch.arange(cache.n_pages, device="cuda").int(), prefix, None, None, return_lse=True)
     assert out.isnan().all() and lse.isnan().all()
+    decode.check()
+
+
+# ---- attention: what a row does not see ---------------------------------------------------------------------
+# batch, q_len, heads, kv_heads, prefix, suffix: a tile for the queries or several, units of one warp or of four
+HIDDEN = [(2, 3, 3, 1, 70, 40), (1, 2, 8, 2, 0, 33), (2, 20, 6, 2, 0, 150), (1, 40, 3, 1, 30, 40), (150, 2, 2, 1, 64, 40),
+          (80, 5, 16, 4, 0, 300), (3, 2, 30, 10, 8192, 65)]
+
+
+@pytest.mark.parametrize("batch,q_len,heads,kv,prefix,suffix", HIDDEN)
+@pytest.mark.parametrize("kind,dtype", [(F16, F16), (BF16, BF16), (I8, F16), (I8, BF16), (E4, F16), (E4, BF16)])
+@pytest.mark.parametrize("where", ["k", "v", "inf"])
+def test_later_tokens_do_not_reach_earlier_queries(b2p, batch, q_len, heads, kv, prefix, suffix, kind, dtype, where):
+    """A non-finite key or value in the last token of a sequence: its last query has it, the others are as without."""
+    page = 16
+    g = gen(batch + q_len)
+    first, each = -(-prefix // page), -(-suffix // page)
+    cache = make_cache(g, first + batch * each, kv, page, kind, dtype)
+    pp = torch.arange(first, device="cuda").int()
+    sp = (first + torch.arange(batch * each, device="cuda")).int().reshape(batch, each)
+    lens = torch.full((batch,), suffix, device="cuda").int()
+    lens[-1] = max(suffix - 7, 1)
+    q = randn(g, batch * q_len, heads * 64).to(dtype)
+    att = decode.PrefixAttention(batch, q_len, heads, kv, prefix, suffix)
+    clean, clean_lse = att(q, cache, pp, prefix, sp, lens, return_lse=True)
+    b, h = batch - 1, kv - 1
+    at = int(lens[b]) - 1
+    spot = (int(sp[b, at // page]), h, at % page)
+    bad = INF if where == "inf" else NAN
+    codes, scale = (cache.k, cache.k_scale) if where == "k" else (cache.v, cache.v_scale)
+    if scale is not None:
+        scale[spot] = bad
+    elif where == "k":
+        codes[spot] = bad
+    else:
+        codes[spot][11] = bad
+    if kind is E4 and where == "v":
+        codes.view(torch.uint8)[spot] = 0x7f  # its codes are NaN too, as written by KVCache.append
+    out, lse = att(q, cache, pp, prefix, sp, lens, return_lse=True)
+    decode.check()
+    shape = (batch, q_len, kv, heads // kv, 64)
+    hit = torch.zeros(shape[:4], dtype=torch.bool, device="cuda")
+    hit[b, -1, h] = True
+    same = (out.view(shape) == clean.view(shape)).all(-1) & (lse.view(shape[:4]) == clean_lse.view(shape[:4]))
+    assert torch.equal(same, ~hit)
+    got = out.view(shape)[b, -1, h]
+    if where == "k" or kind in (I8, E4):
+        assert got.isnan().all() if where != "inf" else not got.isfinite().any()
+    else:  # one channel of the value
+        assert (got[:, 11] == INF).all() if where == "inf" else got[:, 11].isnan().all()
+        got, ref = got.clone(), clean.view(shape)[b, -1, h].clone()
+        got[:, 11] = ref[:, 11] = 0
+        assert torch.equal(got, ref)
+
+
+def test_infinite_values_of_both_signs(b2p):
+    """Infinite values of both signs that one query sees make its channel NaN; of one sign, infinite."""
+    g = gen(5)
+    cache = make_cache(g, 4, 1, 16, F16, F16)
+    cache.v[2, 0, 5, 3] = INF
+    cache.v[2, 0, 6, 3] = -INF
+    cache.v[2, 0, 6, 4] = -INF
+    lens = ints(16 + 16 + 7)
+    q = randn(g, 3, 64).half()
+    out = decode.PrefixAttention(1, 3, 1, 1, 0, 64)(q, cache, None, 0, ints(0, 1, 2, 3).view(1, 4), lens)
+    want, _, _ = attend64(q, cache, ints(), 0, ints(0, 1, 2, 3).view(1, 4), lens.cpu(), 3)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf())
+    assert out[0].isfinite().all() and out[1, 3] == INF and out[2, 3].isnan() and out[2, 4] == -INF
     decode.check()
