@@ -50,7 +50,7 @@ def _raise(name: str, rc: int):
 
 
 _stream = torch._C._cuda_getCurrentRawStream  # of a device index
-_current = torch.cuda.current_device
+_current = torch._C._cuda_getDevice
 
 
 def _on(device: int) -> int:
