@@ -574,7 +574,9 @@ __device__ __forceinline__ bool gather(Mem<NT>& s, const Row<T>& row, const Para
   constexpr int kVec = Row<T>::kVec;
   if (threadIdx.x == 0) s.listed = s.queued = 0;
   __syncthreads();  // (the histogram is done with, too)
-  const float low = least_logit(to, q);
+  // (not -inf, which it is at an infinite temperature: the vectors that a warp loads past its segment read as -inf, and
+  // are real ones of the next warps)
+  const float low = fmaxf(least_logit(to, q), -3.402823466e38f);
   row.template each<false>([&](int j, const uint4& e) {
     if (Row<T>::most(e) >= low) {
       const uint32_t at = atomicAdd(&s.queued, 1u);

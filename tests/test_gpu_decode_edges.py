@@ -123,3 +123,29 @@ def test_infinite_values_of_both_signs(b2p):
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf())
     assert out[0].isfinite().all() and out[1, 3] == INF and out[2, 3].isnan() and out[2, 4] == -INF
     decode.check()
+
+
+# ---- sampling -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
+@pytest.mark.parametrize("vocab", [203, 500, 1000, 20000])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_sample_infinite_temperature(b2p, dtype, vocab, rows):
+    """Every finite logit weighs the same: the filters keep the lowest indices, and the draw goes through them evenly."""
+    logits = (randn(gen(vocab), rows, vocab) * 3).to(dtype)
+    u = (torch.arange(rows, device="cuda") + 0.5) / rows
+    hot = torch.full((rows,), INF, device="cuda")
+    for n in (1, 50, min(2 * vocab // 3, 500)):
+        k = torch.full((rows,), n, device="cuda").int()
+        tokens, logprobs = decode.sample(logits, u, hot, top_k=k)
+        assert torch.equal(tokens, (u.double() * n).int())
+        assert torch.allclose(logprobs, torch.full_like(u, -math.log(n)), atol=1e-5)
+    for part in (0.25, 0.875):
+        kept = math.ceil(vocab * part)  # the tokens before the last one kept weigh less than the part
+        tokens, logprobs = decode.sample(logits, u, hot, top_p=torch.full((rows,), part, device="cuda"))
+        assert torch.equal(tokens, (u.double() * kept).int())
+        assert torch.allclose(logprobs, torch.full_like(u, -math.log(kept)), atol=1e-5)
+    tokens, _ = decode.sample(logits, u, hot)
+    assert torch.equal(tokens, (u.double() * vocab).int())
+    logits[:, :10] = -INF
+    tokens, _ = decode.sample(logits, u, hot, top_k=torch.full((rows,), 150, device="cuda").int())
+    assert torch.equal(tokens, 10 + (u.double() * 150).int())
