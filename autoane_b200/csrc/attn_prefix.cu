@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
   }
 
   const uint32_t ring = smem_u32(s_ring) + (threadIdx.x >> 5) * (Mem::kRing * Mem::kBytes);
-  const uint32_t page_vecs = (uint32_t)a.c.kv_heads << sh;  // vectors of a page
+  const uint32_t page_vecs = (uint32_t)a.c.kv_heads << sh;  // vectors of a page (its bytes may pass 32 bits)
   const uint8_t* k0 = a.c.k + ((long long)kvh << sh) * Mem::kRow + lane * 16;
   const uint8_t* v0 = a.c.v + ((long long)kvh << sh) * Mem::kRow + lane * 16;
   auto page_of = [&](int key) {
@@ -282,8 +282,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
 #pragma unroll
       for (int n = 0; n < kStep / kKeys; ++n) {
         const int at = (key0 + n * kKeys) & ((1 << sh) - 1);  // (a round lies inside one page)
-        const unsigned long long off = (unsigned long long)page_of(key0 + n * kKeys) * (page_vecs * Mem::kRow) +
-                                       (uint32_t)(at * Mem::kRow);
+        const unsigned long long off = ((unsigned long long)page_of(key0 + n * kKeys) * page_vecs + at) * Mem::kRow;
         const int kk = n * kKeys + lane / Mem::kChunks, ch = lane % Mem::kChunks;
         const bool live = whole || key0 + kk < end;
         cp_async_or_zero16(dst + Mem::k_at(kk, ch), k0 + off, live);

@@ -125,6 +125,19 @@ def test_infinite_values_of_both_signs(b2p):
     decode.check()
 
 
+# ---- attention: lengths and sizes -------------------------------------------------------------------------------
+def test_page_of_4_gb(b2p):
+    """A page whose bytes pass 2^32: the second page is read as the second."""
+    kv, page = 32768, 1024
+    cache = decode.KVCache(*(torch.zeros(2, kv, page, 64, dtype=F16, device="cuda") for _ in range(2)))
+    v = randn(gen(12), kv, 64).half()
+    cache.v[1, :, 0] = v
+    q = torch.zeros(1, 64 * kv, dtype=F16, device="cuda")
+    out = decode.PrefixAttention(1, 1, kv, kv, 1, 0)(q, cache, ints(1), 1, None, None)
+    decode.check()
+    assert torch.equal(out.view(kv, 64), v)
+
+
 # ---- sampling -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
 @pytest.mark.parametrize("vocab", [203, 500, 1000, 20000])
