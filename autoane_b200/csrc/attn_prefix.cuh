@@ -107,12 +107,13 @@ __device__ __forceinline__ void join_row(const PrefixArgs& a, int kvh, int r, in
       }
     }
   }
-  const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+  // (a row that sees nothing has no weights; one whose scores are all NaN has no maximum either, but its sum is NaN)
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int token = r / a.group, h = kvh * a.group + r % a.group;
   T* out = static_cast<T*>(a.out) + (long long)token * a.ld_out + h * kKvHeadDim + sub * 4;
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_h2<T>(acc.x * inv, acc.y * inv), pack_h2<T>(acc.z * inv, acc.w * inv));
   if (a.lse && sub == 0)
-    a.lse[(long long)token * a.c.kv_heads * a.group + h] = top == -INFINITY ? -INFINITY : ref + log2f(sum);
+    a.lse[(long long)token * a.c.kv_heads * a.group + h] = sum == 0.f ? -INFINITY : ref + log2f(sum);
 }
 
 }  // namespace b2p

@@ -125,6 +125,25 @@ def test_infinite_values_of_both_signs(b2p):
     decode.check()
 
 
+@pytest.mark.parametrize("prefix,suffix", [(50, 20), (50, 0), (0, 20), (9000, 0), (9000, 300)])
+def test_a_nan_query_has_a_nan_log_sum(b2p, prefix, suffix):
+    """-inf says that a query sees nothing; one whose scores are all NaN has NaN, in the output and the log-sum-exp."""
+    g = gen(6)
+    first, each = -(-prefix // 16), -(-suffix // 16)
+    cache = make_cache(g, first + 2 * each, 1, 16, F16, F16)
+    q = randn(g, 2, 3 * 64).half()
+    q[1, 64:128] = NAN
+    sp = (first + torch.arange(2 * each, device="cuda")).int().view(2, each)
+    att = decode.PrefixAttention(2, 1, 3, 1, prefix, suffix)
+    out, lse = att(q, cache, torch.arange(first, device="cuda").int(), prefix, sp, ints(suffix, suffix),
+                   return_lse=True)
+    bad = torch.zeros(2, 3, dtype=torch.bool, device="cuda")
+    bad[1, 1] = True
+    assert torch.equal(out.view(2, 3, 64).isnan().all(-1), bad) and torch.equal(lse.isnan(), bad)
+    assert lse[~bad].isfinite().all()
+    decode.check()
+
+
 # ---- attention: lengths and sizes -------------------------------------------------------------------------------
 def test_page_of_4_gb(b2p):
     """A page whose bytes pass 2^32: the second page is read as the second."""
