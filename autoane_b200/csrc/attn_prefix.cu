@@ -23,7 +23,7 @@
 // column of S in fp32. A value's scale y_j joins the exponent,
 //   w_j = exp2(s_j log2e + log2 y_j - M), M near the largest of the sums so far,
 // so that o = sum w_j code_j, l = sum w_j / y_j and out = o / l: the one rounding
-// to 16 bit is that of w_j, as without scales, however small the values are.
+// to 16 bit is that of w_j, as without scales, for values down to 2^-73.
 //
 // Bound: for few rows the latency of a unit's loads and of the join; for many the
 // instructions around 16 x 8 tiles that hold 3 rows of 16 (group 3). 256 suffixes
@@ -338,8 +338,11 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 ? 3 : 2)
       if constexpr (KIND != B2P_KV_16) {
         const uint2 ks = lds8(src + Mem::kScale + (8 * j + 2 * t) * 4);
         const uint2 vs = lds8(src + Mem::kScale + (kStep + 8 * j + 2 * t) * 4);
-        // (a key that is not there has scale 0: its weight is 0, and 1 in the place of 1 / 0)
-        const float v0 = vs.x ? __uint_as_float(vs.x) : 1.f, v1 = vs.y ? __uint_as_float(vs.y) : 1.f;
+        // A smaller scale, such as that of a vector of zeros, counts as 2^-80: then neither its logarithm nor its
+        // reciprocal leaves fp32, and beside a scale of 2^30 (2^9 is fp16's most) only weights below 2^-16 of the largest
+        // are lost from l. (A key that is not there has scale 0.)
+        const float y0 = __uint_as_float(vs.x), y1 = __uint_as_float(vs.y);
+        const float v0 = fabsf(y0) < 0x1p-80f ? 0x1p-80f : y0, v1 = fabsf(y1) < 0x1p-80f ? 0x1p-80f : y1;
         kc[0] = __uint_as_float(ks.x) * kScaleLog2;
         kc[1] = __uint_as_float(ks.y) * kScaleLog2;
         vl[0] = log2_sfu(v0);

@@ -192,7 +192,8 @@ int b2p_kv_read(const b2p_kv_cache* cache, const int32_t* slots, int n_tokens, v
  *   out [batch*q_len][ld_out]: softmax(q·Kᵀ/8)·V in the compute dtype
  *   lse (may be NULL) fp32 [batch*q_len][heads]: log2 of the sum of exp, as in
  *       b2p_attention: max·log2(e)/8 + log2(sum)
- * A query that sees nothing gets zeros and -inf. suffix_lens lives on the
+ * A query that sees nothing gets zeros and -inf. In 8-bit caches a value's scale
+ * below 2^-80 (vectors of zeros have one) may count as 2^-80. suffix_lens lives on the
  * device; max_suffix bounds its entries and suffix_pitch >=
  * ceil(max_suffix/page_size). Query head h reads KV head h / (heads/kv_heads).
  * `workspace` holds at least b2p_attention_prefix_workspace() bytes (16-byte

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from autoane_b200 import decode
-from tests.test_gpu_decode import BF16, E4, F16, I8, attend64, gen, make_cache, randn
+from tests.test_gpu_decode import BF16, E4, F16, I8, U, attend64, gen, make_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -142,6 +142,50 @@ def test_a_nan_query_has_a_nan_log_sum(b2p, prefix, suffix):
     assert torch.equal(out.view(2, 3, 64).isnan().all(-1), bad) and torch.equal(lse.isnan(), bad)
     assert lse[~bad].isfinite().all()
     decode.check()
+
+
+# ---- attention: scales ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("prefix", [100, 8192])
+@pytest.mark.parametrize("scale", [0.0, 1e-40])
+def test_values_of_vanishing_scale(b2p, kind, prefix, scale):
+    """A value whose scale is zero or subnormal counts as (next to) zero, whatever its codes, and its weight counts."""
+    g = gen(7)
+    pages = -(-prefix // 64)
+    cache = make_cache(g, pages, 1, 64, kind, F16)
+    cache.v_scale[:, :, ::3] = scale
+    q = randn(g, 4, 64).half()
+    pp = torch.arange(pages, device="cuda").int()
+    att = decode.PrefixAttention(4, 1, 1, 1, prefix, 0)
+    out, lse = att(q, cache, pp, prefix, None, None, return_lse=True)
+    none = torch.zeros(4, 0, dtype=torch.int32, device="cuda")
+    want, wlse, _ = attend64(q, cache, pp, prefix, none, torch.zeros(4, dtype=torch.int32), 1)
+    size = (cache.v.float() * cache.v_scale[..., None]).abs().max()
+    assert ((lse - wlse).abs() <= 1e-4).all()
+    assert ((out - want).abs() <= (2 * U[F16] + prefix * 2.0 ** -25 + 1e-4) * size).all()
+
+
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_weights_of_zero_values_count_beside_large_ones(b2p, kind):
+    """Vectors of zeros (written with the smallest scale) beside values of 2^18: each has its weight in the sum."""
+    n = 128
+    g = gen(8)
+    x = randn(g, n, 3 * 64)
+    x[:, :64] = 0
+    x[:, 64:128] *= 0.02
+    x[:, 128:] *= 2.0 ** 18
+    x[0, 64:128] = 4.0      # the heaviest key, of a large value
+    x[1:, 128:] = 0         # all others have none
+    cache = decode.KVCache.empty(2, 64, 1, kind)
+    cache.append(x.to(BF16), 1, torch.arange(n, device="cuda").int())
+    q = torch.full((1, 64), 0.35, device="cuda").to(BF16)  # key 0 weighs 2^16 times each other: a 500th is theirs
+    pp = ints(0, 1)
+    out, lse = decode.PrefixAttention(1, 1, 1, 1, n, 0)(q, cache, pp, n, None, None, return_lse=True)
+    want, wlse, _ = attend64(q, cache, pp, n, torch.zeros(1, 0, dtype=torch.int32, device="cuda"),
+                             torch.zeros(1, dtype=torch.int32), 1)
+    assert ((lse - wlse).abs() <= 1e-4).all()
+    size = want.abs().max()
+    assert ((out - want).abs() <= (2 * U[BF16] + n * 2.0 ** -25 + 1e-4) * size).all()
 
 
 # ---- attention: lengths and sizes -------------------------------------------------------------------------------
