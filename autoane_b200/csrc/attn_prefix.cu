@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(PrefixArgs a, uint32_t* 
   pdl_enter();
   const int r = blockIdx.x * 8 + (threadIdx.x >> 4);
   if (r >= a.rows) return;
-  const int len = a.max_suffix > 0 ? suffix_len(a, r / (a.q_len * a.group), status) : 0;
+  const int len = a.suffix_lens ? suffix_len(a, r / (a.q_len * a.group), status) : 0;
   join_row<T>(a, blockIdx.y, r, len, threadIdx.x & 15);
 }
 

@@ -226,7 +226,8 @@ class PrefixAttention:
                  suffix_pages: torch.Tensor | None, suffix_lens: torch.Tensor | None, out: torch.Tensor | None = None,
                  return_lse: bool = False):
         """q [batch·q_len, 64·heads]; prefix_pages int32 [ceil(prefix_len/page_size)]; suffix_pages int32
-        [batch, pages]; suffix_lens int32 [batch] (None: no suffixes). Returns out, or (out, lse [batch·q_len, heads])."""
+        [batch, pages]; suffix_lens int32 [batch] (None: no suffixes; lengths above max_suffix or the pages are reported
+        by `check()`). Returns out, or (out, lse [batch·q_len, heads])."""
         n, cols, dev = self.batch * self.q_len, self.heads * HEAD_DIM, cache._dev
         if _rows(q, "q").shape != (n, cols) or q.get_device() != dev or cache.kv_heads != self.kv_heads:
             raise ValueError(f"q must be [{n}, {cols}] on {cache.device}, the cache have {self.kv_heads} KV heads")
@@ -241,14 +242,15 @@ class PrefixAttention:
             if prefix_pages is None or prefix_pages.numel() * cache.page_size < prefix_len:
                 raise ValueError(f"prefix_pages must name {-(-prefix_len // cache.page_size)} pages")
             prefix = _vec(prefix_pages, "prefix_pages", torch.int32, prefix_pages.numel(), dev)
-        if suffix_lens is not None and self.max_suffix:
-            if suffix_pages is None or suffix_pages.dim() != 2 or suffix_pages.shape[0] != self.batch:
-                raise ValueError("suffix_pages must be [batch, pages]")
-            pitch = suffix_pages.shape[1]
-            most = min(self.max_suffix, pitch * cache.page_size)
-            if most:
-                pages = _vec(suffix_pages, "suffix_pages", torch.int32, self.batch * pitch, dev)
-                lens = _vec(suffix_lens, "suffix_lens", torch.int32, self.batch, dev)
+        if suffix_lens is not None:  # (where there is no room for a suffix, the lengths are still checked)
+            lens = _vec(suffix_lens, "suffix_lens", torch.int32, self.batch, dev)
+            if self.max_suffix:
+                if suffix_pages is None or suffix_pages.dim() != 2 or suffix_pages.shape[0] != self.batch:
+                    raise ValueError("suffix_pages must be [batch, pages]")
+                pitch = suffix_pages.shape[1]
+                most = min(self.max_suffix, pitch * cache.page_size)
+                if most:
+                    pages = _vec(suffix_pages, "suffix_pages", torch.int32, self.batch * pitch, dev)
         ld_q = _ld(q)
         if out is None:
             out = torch.empty_like(q) if ld_q == cols else q.new_empty((n, cols))

@@ -195,7 +195,9 @@ int b2p_kv_read(const b2p_kv_cache* cache, const int32_t* slots, int n_tokens, v
  * A query that sees nothing gets zeros and -inf. In 8-bit caches a value's scale
  * below 2^-80 (vectors of zeros have one) may count as 2^-80. suffix_lens lives on the
  * device; max_suffix bounds its entries and suffix_pitch >=
- * ceil(max_suffix/page_size). Query head h reads KV head h / (heads/kv_heads).
+ * ceil(max_suffix/page_size). With max_suffix = 0 suffix_pages is not read, and
+ * suffix_lens may be NULL; lengths that are given must be 0, as checked on the
+ * device. Query head h reads KV head h / (heads/kv_heads).
  * `workspace` holds at least b2p_attention_prefix_workspace() bytes (16-byte
  * aligned) for sizes that are at least this call's in each argument; calls that
  * share one must be ordered by their stream. Results repeat bit for bit. */

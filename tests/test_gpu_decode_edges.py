@@ -189,6 +189,26 @@ def test_weights_of_zero_values_count_beside_large_ones(b2p, kind):
 
 
 # ---- attention: lengths and sizes -------------------------------------------------------------------------------
+def test_lengths_that_the_plan_leaves_no_room_for(b2p):
+    """Suffix lengths above what the object was made for are reported, where that is none as well."""
+    cache = make_cache(gen(10), 6, 1, 16, F16, F16)
+    q = randn(gen(11), 2, 64).half()
+    sp, pp = ints(2, 3, 4, 5).view(2, 2), ints(0, 1)
+    att = decode.PrefixAttention(2, 1, 1, 1, 32, 0)
+    plain = att(q, cache, pp, 32, None, None)
+    assert torch.equal(att(q, cache, pp, 32, sp, ints(0, 0)), plain)
+    decode.check()
+    att(q, cache, pp, 32, sp, ints(0, 9))
+    with pytest.raises(decode.B2PError):
+        decode.check()
+    roomy = decode.PrefixAttention(2, 1, 1, 1, 32, 64)
+    roomy(q, cache, pp, 32, sp[:, :0], ints(3, 0))  # no pages for them
+    with pytest.raises(decode.B2PError):
+        decode.check()
+    assert torch.equal(roomy(q, cache, pp, 32, sp[:, :0], ints(0, 0)), plain)
+    decode.check()
+
+
 def test_page_of_4_gb(b2p):
     """A page whose bytes pass 2^32: the second page is read as the second."""
     kv, page = 32768, 1024
