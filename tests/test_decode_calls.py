@@ -73,3 +73,11 @@ def test_workspace_of_another_device_is_refused(calls, monkeypatch):
     with pytest.raises(ValueError, match="workspace"):
         att(on_1(1, 64), cache_1(), vec(1), 8, None, None)
     assert not calls
+
+
+def test_large_pitches():
+    """A pitch beyond the library's 32 bits is refused, not cut off."""
+    far = torch.empty_strided((2, 64), (1 << 31, 1), dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="pitch"):
+        decode._ld(far)
+    assert decode._ld(torch.empty_strided((2, 64), ((1 << 31) - 8, 1), device="meta")) == (1 << 31) - 8
