@@ -78,7 +78,9 @@ def _vec(t, name: str, dtype, n: int, device: int):
 
 
 def _ld(t: torch.Tensor) -> int:
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if t.shape[0] <= 1:  # no second row: any pitch that keeps 16 bytes does
+        return t.shape[1] + -t.shape[1] % 8
+    ld = t.stride(0)
     if ld >= 1 << 31:  # (ctypes would cut it off)
         raise ValueError(f"a row pitch of {ld} elements is more than the library takes (2^31 - 1)")
     return ld

@@ -81,3 +81,11 @@ def test_large_pitches():
     with pytest.raises(ValueError, match="pitch"):
         decode._ld(far)
     assert decode._ld(torch.empty_strided((2, 64), ((1 << 31) - 8, 1), device="meta")) == (1 << 31) - 8
+
+
+def test_pitch_of_one_row():
+    """The pitch of a matrix of one row is of no account; any other's is passed on."""
+    one = torch.empty(1, 1603, device="meta")
+    assert decode._ld(one[:, :1600]) == 1600
+    assert decode._ld(one) >= 1603 and decode._ld(one) % 8 == 0
+    assert decode._ld(torch.empty(3, 1603, device="meta")[:, :1600]) == 1603

@@ -221,6 +221,29 @@ def test_page_of_4_gb(b2p):
     assert torch.equal(out.view(kv, 64), v)
 
 
+def test_one_row_of_any_pitch(b2p):
+    """The pitch of a matrix of one row is of no account."""
+    g = gen(13)
+    wide = randn(g, 1, 25 * 64 + 3).half()
+    table, pos = decode.rope_table(8), ints(5)
+    one, two = decode.KVCache.empty(1, 16, 5), decode.KVCache.empty(1, 16, 5)
+    qkv = wide[:, :25 * 64]
+    a = one.append(qkv, 15, ints(3), pos, table)
+    b = two.append(qkv.clone(), 15, ints(3), pos, table)
+    assert torch.equal(a, b)
+    k = [torch.empty(1, 323, dtype=F16, device="cuda")[:, :320] for _ in range(2)]
+    one.read(ints(3), F16, *k)
+    assert all(torch.equal(x, y) for x, y in zip(k, two.read(ints(3), F16)))
+    q = torch.empty(1, 15 * 64 + 1, dtype=F16, device="cuda")[:, :960]
+    q.copy_(a)
+    att = decode.PrefixAttention(1, 1, 15, 5, 16, 0)
+    y = torch.empty(1, 967, dtype=F16, device="cuda")[:, :960]
+    one.k[:], one.v[:], one.k_scale[:], one.v_scale[:] = 1, 2, 0.1, 0.1
+    att(q, one, ints(0), 16, None, None, out=y)
+    assert torch.equal(y, att(a, one, ints(0), 16, None, None))
+    decode.check()
+
+
 # ---- sampling -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
 @pytest.mark.parametrize("vocab", [203, 500, 1000, 20000])
