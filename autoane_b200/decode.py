@@ -4,7 +4,8 @@ sequences share a long prefix, and sampling.
 A thin layer over b2p_kv_append, b2p_kv_read, b2p_attention_prefix and
 b2p_sample (include/b2p.h has their definitions) for torch tensors. All work
 goes to torch's current stream of the current device, which has to be the
-tensors' own (the library launches there); nothing synchronises.
+tensors' own (the library launches there); nothing synchronises. There is no
+backward pass: under autograd, inputs that require a gradient are refused.
 Argument errors raise `B2PError` (from the library) or `ValueError` (shapes and
 types of the tensors). Indices on the device (slots, positions, page ids,
 lengths) are checked there: `check()` raises if any was out of range.
@@ -65,6 +66,8 @@ def _on(device: int) -> int:
 def _rows(t: torch.Tensor, name: str, dtypes=_DTYPE) -> torch.Tensor:
     if t.dim() != 2 or t.dtype not in dtypes or not t.is_cuda or (t.stride(1) != 1 and t.shape[1] > 1):
         raise ValueError(f"{name} must be a CUDA matrix of {[str(d) for d in dtypes]} with contiguous rows")
+    if t.requires_grad and torch.is_grad_enabled():  # (what comes back would have no history, without a word)
+        raise ValueError(f"{name} requires a gradient and these operators have none: detach it, or call under no_grad")
     return t
 
 

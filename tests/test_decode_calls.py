@@ -75,6 +75,21 @@ def test_workspace_of_another_device_is_refused(calls, monkeypatch):
     assert not calls
 
 
+def test_tensors_that_require_a_gradient_are_refused(calls, monkeypatch):
+    """The operators have no backward pass: under autograd their inputs may not require one."""
+    monkeypatch.setattr(decode, "_current", lambda: 1)
+    logits, u = on_1(2, 10, dtype=torch.float32).requires_grad_(), vec(2, torch.float32)
+    with pytest.raises(ValueError, match="gradient"):
+        decode.sample(logits, u)
+    with pytest.raises(ValueError, match="gradient"):
+        cache_1().append(on_1(2, 192).requires_grad_(), 1, vec(2))
+    assert not calls
+    with torch.no_grad():
+        decode.sample(logits, u)
+    decode.sample(logits.detach(), u)
+    assert len(calls) == 2
+
+
 def test_large_pitches():
     """A pitch beyond the library's 32 bits is refused, not cut off."""
     far = torch.empty_strided((2, 64), (1 << 31, 1), dtype=torch.float16, device="meta")
