@@ -105,7 +105,8 @@ def rope_table(positions: int, rot: int = HEAD_DIM, theta: float = 10000.0, scal
     `scale` s divides every angle by s (position interpolation); with yarn = (trained_positions, fast, slow) a pair
     that makes more than `fast` turns over trained_positions keeps its angle, one that makes fewer than `slow` is
     divided by s, those between are blended linearly in the pair index, and cosines and sines carry the factor
-    0.1·ln(s) + 1 (the attention temperature of that scheme)."""
+    0.1·ln(s) + 1 (the attention temperature of that scheme: YaRN, Peng, Quesnelle, Fan and Shippole, 2023, from
+    which the steps are)."""
     if rot % 16 or not 0 < rot <= HEAD_DIM:
         raise ValueError(f"rot must be 16, 32, 48 or {HEAD_DIM} (got {rot})")
     i = torch.arange(rot // 2, dtype=torch.float64)
@@ -114,8 +115,9 @@ def rope_table(positions: int, rot: int = HEAD_DIM, theta: float = 10000.0, scal
     if yarn is not None:
         trained, fast, slow = yarn
         pair = lambda turns: rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
-        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot // 2 - 1)
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
         blend = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        blend[i >= pair(slow)] = 1.0  # (the first pair, too, where none makes as many turns)
         freq = freq * (1 - blend) + freq / scale * blend
         size = 0.1 * math.log(scale) + 1.0 if scale > 1 else 1.0
     else:

@@ -1,5 +1,7 @@
 """What the decoding calls refuse or pass on before any GPU work, with tensors that stand in for another GPU's: no
 launch is made."""
+import math
+
 import pytest
 import torch
 
@@ -104,3 +106,27 @@ def test_pitch_of_one_row():
     assert decode._ld(one[:, :1600]) == 1600
     assert decode._ld(one) >= 1603 and decode._ld(one) % 8 == 0
     assert decode._ld(torch.empty(3, 1603, device="meta")[:, :1600]) == 1603
+
+
+@pytest.mark.parametrize("rot,theta,trained,fast,slow", [
+    (64, 10000.0, 2048, 32.0, 1.0), (64, 10000.0, 1 << 17, 32.0, 1.0), (16, 10000.0, 32768, 32.0, 1.0),
+    (32, 500.0, 8192, 32.0, 2.0), (64, 10000.0, 4, 32.0, 1.0), (16, 100000.0, 1 << 20, 2.0, 1.0)])
+def test_yarn_keeps_and_divides_by_turns(rot, theta, trained, fast, slow):
+    """A pair that makes more than `fast` turns over the trained positions keeps its angle, one that makes fewer than
+    `slow` is divided by the scale, and those between go from the one to the other without a step back."""
+    scale = 8.0
+    size = 0.1 * math.log(scale) + 1
+    t = decode.rope_table(2, rot, theta, scale, (trained, fast, slow), device="cpu").double()[1] / size
+    freq = theta ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+    turns = trained * freq / (2 * math.pi)
+    part = torch.atan2(t[:, 1], t[:, 0]) / freq  # of the plain angle
+    tol = 1e-6 / freq
+    assert ((part - 1).abs() <= tol)[turns > fast].all()
+    assert ((part - 1 / scale).abs() <= tol)[turns < slow].all()
+    # the whole ramp: from 0 at the last pair above `fast` to 1 at the first one below `slow`
+    at = lambda n: rot * math.log(trained / (n * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+    lo, hi = max(math.floor(at(fast)), 0), math.ceil(at(slow))
+    for i in range(rot // 2):
+        if slow <= turns[i] <= fast and hi > lo:
+            blend = min(max((i - lo) / (hi - lo), 0.0), 1.0)
+            assert abs(part[i] - (1 - blend + blend / scale)) <= tol[i], (i, part[i])
