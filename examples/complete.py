@@ -41,10 +41,11 @@ def gemm(x: torch.Tensor, w: torch.Tensor, out_f32: bool = False) -> torch.Tenso
 class Completer:
     """`weights`: lists by layer of Wq, Wk, Wv, Wo, W1, W2, W3 [out, in] (adapters merged); `rms` [2·layers + 1, dim]:
     the attention's and the feed-forward's norm of every layer, then the last one; `embed` [vocab, dim]; `head`
-    [tokens, dim]: the rows of the embedding that a token may be drawn from."""
+    [tokens, dim]: the rows of the embedding that a token may be drawn from, and `ids` which rows of `embed` they are (a
+    compacted vocabulary's ids; None: the first ones, in order)."""
 
     def __init__(self, cfg: Config, weights: dict, rms, embed, head, batch: int, max_prompt: int, max_new: int,
-                 kv: torch.dtype = torch.int8, dtype: torch.dtype = torch.float16):
+                 kv: torch.dtype = torch.int8, dtype: torch.dtype = torch.float16, ids=None):
         put = lambda a: torch.as_tensor(a).to("cuda", dtype).contiguous()  # noqa: E731
         self.cfg, self.batch, self.max_prompt, self.max_new, self.dtype = cfg, batch, max_prompt, max_new, dtype
         layers = range(cfg.nlayers)
@@ -54,6 +55,9 @@ class Completer:
         self.o, self.down = w["Wo"], w["W2"]
         self.rms = torch.as_tensor(rms).to("cuda", torch.float32)
         self.embed, self.head = torch.as_tensor(embed).to("cuda", torch.float32), put(head)
+        self.ids = torch.arange(len(head), device="cuda") if ids is None else torch.as_tensor(ids).to("cuda", torch.long)
+        if self.ids.shape != (self.head.shape[0],):
+            raise ValueError("ids must name an embedding row for each row of head")
 
         prompt_pages, own_pages = -(-max_prompt // PAGE), -(-max_new // PAGE)
         self.cache = [decode.KVCache.empty(prompt_pages + batch * own_pages, PAGE, cfg.kv_heads, kv) for _ in layers]
@@ -120,15 +124,15 @@ class Completer:
         return self._logits(x)
 
     def complete(self, prompt: torch.Tensor, new: int, u: torch.Tensor, **filters) -> torch.Tensor:
-        """`new` tokens for every sample, drawn by u [new, batch]: indices into `head`'s rows, [batch, new]. The filters
-        are `sample`'s."""
+        """`new` tokens for every sample after a prompt of `embed`'s rows, drawn by u [new, batch]: indices into `head`'s
+        rows, [batch, new]. The filters are `sample`'s."""
         logits = self.prefill(prompt).expand(self.batch, -1).contiguous()
         out = []
         for i in range(new):
             tokens, _ = decode.sample(logits, u[i], **filters)
             out.append(tokens)
             if i + 1 < new:
-                logits = self.step(tokens)
+                logits = self.step(self.ids[tokens.long()])
         return torch.stack(out, 1)
 
 
