@@ -103,16 +103,17 @@ __device__ __forceinline__ uint2 lds8(uint32_t addr) {
   return v;
 }
 
+// (ordinary loads: the read-only path is for what no kernel writes while this one runs, and the one before may)
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
   if constexpr (N == 2) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
     w[0] = x.x;
     w[1] = x.y;
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      const uint4 x = reinterpret_cast<const uint4*>(p)[i];
       w[4 * i] = x.x;
       w[4 * i + 1] = x.y;
       w[4 * i + 2] = x.z;

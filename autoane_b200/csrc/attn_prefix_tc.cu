@@ -305,27 +305,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(PrefixArg
     const uint32_t kv_base = smem_u32(smem + TcSmem::kKV);
     const uint32_t raw_base = smem_u32(smem + TcSmem::kRawOff);
     const uint32_t scale_base = smem_u32(smem + TcSmem::kRawScale);
-    // page of a key of the part, negative past its end or where the list is wrong; and the key's vector index there
-    auto page_of = [&](int key) -> int {
-      const int page = __ldg(a.prefix_pages + ((first + min(key, nkeys - 1)) >> sh));
-      const bool bad = (unsigned)page >= (unsigned)a.c.n_pages;
-      if (bad) atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
-      return key < nkeys && !bad ? page : -1;
+    // Pages of four keys `step` apart, as the list has them; then, when they have arrived, negative past the part's end or
+    // where the list is wrong. And a key's vector index in its page.
+    struct Pages {
+      int of[4];
+    };
+    auto pages = [&](int key, int step) {
+      Pages p;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p.of[i] = a.prefix_pages[(first + min(key + i * step, nkeys - 1)) >> sh];
+      return p;
+    };
+    auto checked = [&](Pages p, int key, int step) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool bad = (unsigned)p.of[i] >= (unsigned)a.c.n_pages;
+        if (bad) atomicCAS(status, 0u, (uint32_t)DEV_BAD_ARGS);
+        if (bad || key + i * step >= nkeys) p.of[i] = -1;
+      }
+      return p;
     };
     auto vec_at = [&](int page, int key) { return a.c.vec(max(page, 0), kvh, (first + key) & mask); };
     if constexpr (Q8) {
       // one cp.async group a stage; a thread widens the pieces that it loaded itself
-      struct Pages {
-        int of[4];
-      };
-      auto pages = [&](int n) {
-        Pages p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p.of[i] = page_of(n * kStageKeys + i * 32 + (tid >> 2));
-        return p;
-      };
+      auto stage_pages = [&](int n) { return pages(n * kStageKeys + (tid >> 2), 32); };
       // Of each of its four keys a thread loads 16 codes of K and V, and the first of the four threads the scales.
-      auto load = [&](int n, const Pages& p) {
+      auto load = [&](int n, const Pages& ids) {
+        const Pages p = checked(ids, n * kStageKeys + (tid >> 2), 32);
         const uint32_t raw = raw_base + (n % kRaw) * kTileBytes;
         const uint32_t sc = scale_base + ((n % kRaw) * 2 * kStageKeys + (tid >> 2)) * 4;
 #pragma unroll
@@ -343,13 +349,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(PrefixArg
         cp_async_commit();
       };
       {
-        const Pages p0 = pages(0), p1 = pages(1), p2 = pages(2);  // (past the end: zeros)
+        const Pages p0 = stage_pages(0), p1 = stage_pages(1), p2 = stage_pages(2);  // (past the end: zeros)
         load(0, p0);
         load(1, p1);
         load(2, p2);
       }
       for (int n = 0; n < stages; ++n) {
-        const Pages next = pages(n + kRaw);  // (the page ids arrive meanwhile)
+        const Pages next = stage_pages(n + kRaw);  // (the page ids arrive meanwhile)
         const int st = n % kStages;
         if (!__all_sync(~0u, mbar_wait_paused<500>(&kv_empty[st], ((n / kStages) & 1) ^ 1u, abort_flag, status,
                                         DEV_TIMEOUT_PRODUCER)))
@@ -411,15 +417,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(PrefixArg
           const uint32_t kt = kv_base + st * 2 * kTileBytes;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            int pages[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pages[i] = page_of(n * kStageKeys + (h * 4 + i) * 16 + (tid >> 3));
+            const int key = n * kStageKeys + h * 64 + (tid >> 3);
+            const Pages p = checked(pages(key, 16), key, 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int row = (h * 4 + i) * 16 + (tid >> 3), ch = tid & 7;
-              const long long off = vec_at(pages[i], n * kStageKeys + row) * 128 + ch * 16;
-              cp_async16_or_zero(kt + swz(row, ch), a.c.k + off, pages[i] >= 0);
-              cp_async16_or_zero(kt + kTileBytes + swz(row, ch), a.c.v + off, pages[i] >= 0);
+              const long long off = vec_at(p.of[i], n * kStageKeys + row) * 128 + ch * 16;
+              cp_async16_or_zero(kt + swz(row, ch), a.c.k + off, p.of[i] >= 0);
+              cp_async16_or_zero(kt + kTileBytes + swz(row, ch), a.c.v + off, p.of[i] >= 0);
             }
           }
         }

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(AppendArgs a, uin
     if (turns && MODE == ROPE_PAIRS) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float4 w = __ldg(tab + l * 2 + i);
+        const float4 w = tab[l * 2 + i];
         c[4 * i] = c[4 * i + 1] = w.x;
         c[4 * i + 2] = c[4 * i + 3] = w.z;
         s[4 * i] = -w.y;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(AppendArgs a, uin
       partner = second ? lane - half_lanes : lane + half_lanes;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 w = __ldg(tab + (second ? l - half_lanes : l) * 4 + i);
+        const float4 w = tab[(second ? l - half_lanes : l) * 4 + i];
         c[2 * i] = w.x;
         c[2 * i + 1] = w.z;
         s[2 * i] = second ? w.y : -w.y;

@@ -1,6 +1,7 @@
 """What the decoding calls refuse or pass on before any GPU work, with tensors that stand in for another GPU's: no
 launch is made."""
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -130,3 +131,14 @@ def test_yarn_keeps_and_divides_by_turns(rot, theta, trained, fast, slow):
         if slow <= turns[i] <= fast and hi > lo:
             blend = min(max((i - lo) / (hi - lo), 0.0), 1.0)
             assert abs(part[i] - (1 - blend + blend / scale)) <= tol[i], (i, part[i])
+
+
+def test_kernels_read_their_inputs_by_ordinary_loads():
+    """These kernels start while the one before them still runs (programmatic launch), and wait for it before they read
+    what it writes. The read-only path (ld.global.nc) is for data that nothing writes while a kernel runs: its loads
+    may come from before the wait."""
+    csrc = Path(decode.__file__).parent / "csrc"
+    names = ["decode.cuh", "kv_cache.cu", "attn_prefix.cuh", "attn_prefix.cu", "attn_prefix_tc.cu", "sample.cu"]
+    for name in names:
+        text = (csrc / name).read_text()
+        assert not any(w in text for w in ("__ldg", "__restrict__", "global.nc")), name
