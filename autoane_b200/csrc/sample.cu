@@ -17,13 +17,19 @@
 //             to gather: a histogram of one entry a thread. They are sorted, and
 //             top-p, min-p and the draw go by that list alone.
 //   top-p     (without top-k) A histogram of the weights; the tokens of the bin
-//             where the cut lies are gathered and sorted.
+//             where the cut lies are gathered and sorted. The vectors that may hold
+//             such a token, or a likelier one, are queued first.
 //   the rest  Sums of the kept weights by warp, each with a segment of the row;
 //             the warp that has the drawn sum walks through its segment.
-// A list of more than 2048 tokens (many equal logits) is cut by refining the
-// histogram instead (long_row). Bound: reading the logits; in practice, for few
-// rows the latency of the passes, for many that of the second one's reads from L2 at
-// 32 warps an SM (issue 35%, the exponential's unit 30% busy).
+// A list of more than 2048 tokens (many equal logits), or a queue of more vectors, is
+// left for refining the histogram (long_row): six more passes over the row, a token a
+// load. A nucleus comes to that where its tokens lie in more than 2048 vectors, as over a
+// whole vocabulary at ordinary temperatures. Measured, normal logits of deviation 2.7,
+// top-p 0.9 at T 0.7 (queued) / T 1 (long): a row of 49152 in 32 bit 32 / 125 us, 33 rows
+// 35 / 133, 256 rows in 16 bit 62 / 245.
+// Bound: reading the logits; in practice, for few rows the latency of the passes, for
+// many that of the second one's reads from L2 at 32 warps an SM (issue 35%, the
+// exponential's unit 30% busy).
 // Measured: a row of 49152 (top-k 50) 10 us, 33 rows of 16893 (top-p 0.95) 25 us, 256
 // rows of 49152 in 16 bit (top-k 200, top-p, min-p) 18 us, 1024 rows of 32000 in 32 bit
 // (unfiltered) 60 us, 2.2 TB/s. (A row held in the registers of a cluster of CTAs, read
@@ -125,7 +131,7 @@ struct Found {  // a bin, and the sums before it
 template <int NT>
 struct Scan {
   u64 c[NT / 32], w[NT / 32];
-  Found found[3];  // bin kBins before each use
+  Found found;  // bin kBins before each use
 };
 
 // A histogram's running sums: each thread has those before its kBins / NT bins.
@@ -159,17 +165,17 @@ __device__ __forceinline__ void scan_bins(Scan<NT>& s, const uint32_t* count, co
     w += s.w[k];
   }
 }
-// The first bin at which the measure (counts, or weights) reaches `aim` (> 0), into found[slot] after the next barrier;
-// c, w: scan_bins' sums.
+// The first bin at which the measure (counts, or weights) reaches `aim` (> 0), into found after the next barrier; c, w:
+// scan_bins' sums.
 template <int NT>
 __device__ __forceinline__ void find_bin(Scan<NT>& s, const uint32_t* count, const u64* weight, u64 c, u64 w,
-                                         bool by_count, u64 aim, int slot) {
+                                         bool by_count, u64 aim) {
   constexpr int kEach = kBins / NT;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int b = threadIdx.x * kEach + i;
     const u64 nc = c + count[b], nw = w + weight[b];
-    if (nc > c && (by_count ? c : w) < aim && (by_count ? nc : nw) >= aim) s.found[slot] = {b, c, w};  // one bin at most
+    if (nc > c && (by_count ? c : w) < aim && (by_count ? nc : nw) >= aim) s.found = {b, c, w};  // one bin at most
     c = nc;
     w = nw;
   }
@@ -257,11 +263,11 @@ __device__ Cut long_cut(LongMem<NT>& s, const T* x, int vocab, const Params& q, 
     long_histogram<NT, T>(s, x, vocab, q, prefix, above, above == 5 ? 5 : 10);
     u64 c, w;
     scan_bins<NT>(s.scan, s.count, s.weight, c, w);
-    if (threadIdx.x == 0) s.scan.found[0] = {kBins, 0, 0};
+    if (threadIdx.x == 0) s.scan.found = {kBins, 0, 0};
     __syncthreads();
-    find_bin<NT>(s.scan, s.count, s.weight, c + c0, w + w0, by_count, aim, 0);
+    find_bin<NT>(s.scan, s.count, s.weight, c + c0, w + w0, by_count, aim);
     __syncthreads();
-    const Found f = s.scan.found[0];
+    const Found f = s.scan.found;
     if (f.bin == kBins) {  // (on the first level only)
       kept = 0;
       for (int i = 0; i < NT / 32; ++i) kept += s.scan.w[i];
