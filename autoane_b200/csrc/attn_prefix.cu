@@ -25,6 +25,12 @@
 // so that o = sum w_j code_j, l = sum w_j / y_j and out = o / l: the one rounding
 // to 16 bit is that of w_j, as without scales, for values down to 2^-73.
 //
+// The weights are rounded to the compute dtype, here and in attn_prefix_tc.cu: the
+// tensor cores take 16-bit pairs, and weights in two parts would double the second
+// product. l is summed before the rounding. Beside the output's own rounding this makes
+// the error against 64 bits 0.0023 (bf16) or 0.00030 (fp16) of the output's size, with
+// weights in 32 bits 0.0017 and 0.00021.
+//
 // Bound: for few rows the latency of a unit's loads and of the join; for many the
 // instructions around 16 x 8 tiles that hold 3 rows of 16 (group 3). 256 suffixes
 // of up to 512 int8 keys, 5 KV heads: 22 us beside 10 us of reading; 8 sequences

@@ -19,7 +19,7 @@
 // full are spread over the SM's four sub-partitions, and with 64 rows or fewer the
 // upper 16 lanes of each quarter are left out. Measured: 768 rows of 5 KV heads over
 // 32768 int8 keys 70 us (28 us of exponentials; two warps share a scheduler's unit
-// and weigh at 68% of its rate), 80 rows of 6 over 4001 16-bit keys 12.5 us, 64 rows
+// and weigh at 68% of its rate), 320 rows of 6 over 4001 16-bit keys 12.5 us, 64 rows
 // of 12 over 8192 e4m3 keys 16 us.
 //
 // ref need not be the maximum: any number near it gives the same quotient. It is
@@ -30,7 +30,9 @@
 //
 // 8-bit caches: a key's scale multiplies its column of S in fp32 (the log-sum-exp
 // stays exact to fp32). A value's scale is 2^e·f, f in [1, 2): 2^e goes into the
-// widened value, exactly, and f into w before its one rounding; the sum of the
+// widened value, exactly but for e4m3 codes under fp16 that fall below 2^-24 (they are
+// off by 2^-25 at most, as an fp16 output of their size would be), and f into w before
+// its one rounding; the sum of the
 // weights is taken without it. S is read as 16 lanes x 256 bit, which gives a
 // thread four rows and a quarter of the columns: a column's factors are read from
 // shared memory once for four scores.
