@@ -33,7 +33,7 @@
 //
 // Bound: for few rows the latency of a unit's loads and of the join; for many the
 // instructions around 16 x 8 tiles that hold 3 rows of 16 (group 3). 256 suffixes
-// of up to 512 int8 keys, 5 KV heads: 22 us beside 10 us of reading; 8 sequences
+// of up to 512 int8 keys, 5 KV heads: 23 us beside 7 us of reading; 8 sequences
 // over 1023 + 129 keys: 9 us with the join.
 #include <cstdint>
 #include <type_traits>

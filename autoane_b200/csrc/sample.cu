@@ -28,7 +28,7 @@
 // top-p 0.9 at T 0.7 (queued) / T 1 (long): a row of 49152 in 32 bit 32 / 125 us, 33 rows
 // 35 / 133, 256 rows in 16 bit 62 / 245.
 // Bound: reading the logits; in practice, for few rows the latency of the passes, for
-// many that of the second one's reads from L2 at 32 warps an SM (issue 35%, the
+// many that of the second one's reads from L2 at 32 warps an SM (issue 31%, the
 // exponential's unit 30% busy).
 // Measured: a row of 49152 (top-k 50) 10 us, 33 rows of 16893 (top-p 0.95) 25 us, 256
 // rows of 49152 in 16 bit (top-k 200, top-p, min-p) 18 us, 1024 rows of 32000 in 32 bit
